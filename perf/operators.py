@@ -262,7 +262,8 @@ def _prompt(s):
 def _scale_of(most):
     """The smallest power of two 2^e, -40 <= e <= 40, with 448 * 2^e >= most."""
     m, x = torch.frexp(most)
-    return torch.exp2(torch.where(m <= 0.875, x - 9, x - 8).clamp(-40, 40).float())
+    e = torch.where(m <= 0.875, x - 9, x - 8).clamp(-40, 40)
+    return torch.exp2(torch.where(most > 0, e, -40).float())
 
 
 def _store(s):
