@@ -70,6 +70,14 @@ SIGNATURES = {
     "v1x_route_pages": [P, I64, P, P, P, I32, I64, I64, P, P, I64, P, I64, I32, I64, P],
     "v1x_gather_slots": [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64,
                          P],
+    "v1x_latent_attention_workspace": [I64, I64, I64, I64],
+    "v1x_latent_attention": [P, I64, I64, P, I64, I64, P, I64, P, I64, I64, P, I64, I64, I64, I64, F32, I32, P, P, P,
+                             I64, P, P],
+    "v1x_prompt_attention": [P, I64, I64, P, I64, I64, P, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, F32, I32, P,
+                             P, P, P],
+    "v1x_kv8_store": [P, P, P, P, I64, I64, P, I64, I64, P, I64, I64, I32, I64, P, I64, I64, P, P, I64, P],
+    "v1x_kv8_attend_workspace": [I64, I64, I64, I64],
+    "v1x_kv8_attend": [P, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P, I64, I64, F32, I32, P, P, P, I64, P],
     "v1x_build_workspace_bytes": [I64],
     "v1x_build_buckets": [P, I64, P, P, P, P, P, P, P, P, I64, P],
     "v1x_build_buckets_noalloc": [P, I64, P, P, P, P, P, P, P, I64, P],
@@ -87,7 +95,8 @@ SIGNATURES = {
                          I64, P, P, P, P, P, P, P, P, P, P, P, I64, P, I64, I64, P, P],
 }
 # entry points whose return type is not int
-RESTYPES = {"v1x_last_error": ctypes.c_char_p, "v1x_build_workspace_bytes": ctypes.c_int64}
+RESTYPES = {"v1x_last_error": ctypes.c_char_p, "v1x_build_workspace_bytes": ctypes.c_int64,
+            "v1x_latent_attention_workspace": ctypes.c_int64, "v1x_kv8_attend_workspace": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib = None

@@ -1,0 +1,44 @@
+// Shared pieces of the attention kernels: 16-bit element types (1 bf16, 2 f16,
+// the codes of v1x.h) and their conversions.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace v1x {
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <typename T>
+__device__ __forceinline__ float2 to_float2(uint32_t two);
+template <>
+__device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t two) {
+  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&two));
+}
+template <>
+__device__ __forceinline__ float2 to_float2<__half>(uint32_t two) {
+  return __half22float2(*reinterpret_cast<__half2*>(&two));
+}
+
+// two floats rounded to nearest even, the first in the low half
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+__device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace attn
+}  // namespace v1x

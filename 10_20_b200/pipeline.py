@@ -35,6 +35,7 @@ from . import _lib
 from . import kernels as K
 from . import query_fused, scoring
 from .gather import _gather_impl
+from .latent_attention import attend_slots
 from .sharding import row_bytes
 
 
@@ -49,14 +50,18 @@ class SelectionStep:
 
     def __init__(self, case, gather: bool = True, gather_v: bool = False, fused_route_pages: bool = True,
                  keep_logits: bool = False, ratio=None, expand: bool = False, budget=None,
-                 fused: bool = True, score_ctas: int = 0):
+                 fused: bool = True, score_ctas: int = 0, attention=None):
         """ratio=None: the fixed page budget take = min(pages, budget) (the
         reference's BudgetMetadata; budget an int32 device tensor of one element,
         by default holding case.take, which bounds it); ratio=(num, den): the
         reference's default take rule min(pages, max(ceil(pages*num/den),
         ceil(topk/64))).  expand: also write the x4 expanded logical positions
         ([B, 4*topk+64], -1 padded).  score_ctas > 0 caps the centre scorer's
-        grid (for small batches stepped many at a time)."""
+        grid (for small batches stepped many at a time).  attention: (q, scale)
+        -- each run then attends the absorbed queries q [B, heads, D] over the
+        selected rows of the latent pool where they lie
+        (latent_attention.attend_slots, the first 512 of D the values), after the
+        selection; `attended` holds (out, lse).  q is read at every run."""
         c = self.case = case
         d = c.lens.device
         B = c.B
@@ -109,6 +114,12 @@ class SelectionStep:
             self.scores = None
         self.status = torch.zeros(1, dtype=torch.int32, device=d)
         self.score_ctas = int(score_ctas)
+        self.attention = attention
+        if attention is not None:
+            _lib.require(c.latent is not None, "attention needs a case with a latent pool")
+            aq = attention[0]
+            self.attended = (torch.empty((B, aq.shape[1], 512), dtype=aq.dtype, device=d),
+                             torch.empty((B, aq.shape[1]), dtype=torch.float32, device=d))
 
     # -- the step ------------------------------------------------------------
     def _centres(self, rs):
@@ -175,6 +186,10 @@ class SelectionStep:
                      self.kv2[rs] if self.gather_v else None, n, c.topk, 0, *lat.stride(),
                      *(lat.stride() if self.gather_v else (0, 0, 0)), self.physical.stride(0))
 
+    def _attend(self):
+        q, scale = self.attention
+        attend_slots(q, self.case.latent, None, self.physical, scale, out=self.attended[0], lse=self.attended[1])
+
     def run(self, marks=None):
         """Launch the step on the current stream.  marks: a list that receives
         (stage name, CUDA event recorded after the stage) -- a per-stage time
@@ -198,6 +213,9 @@ class SelectionStep:
             if self.gather:
                 self._gather(rs)
                 mark("gather")
+            if self.attention is not None:
+                self._attend()
+                mark("attend")
             return
         # query metadata with the fixed page budget + sink/tail staging, one launch
         K.query_prepare(c.lens, c.native_table, self.fine_lens, self.takes, self.dg_lens, self.center_lens,
@@ -216,6 +234,9 @@ class SelectionStep:
         if self.gather:
             self._gather(rs)
             mark("gather")
+        if self.attention is not None:
+            self._attend()
+            mark("attend")
 
     def capture(self, warmup: int = 2):
         s = torch.cuda.Stream(device=self.case.lens.device)
@@ -239,8 +260,8 @@ class SelectionStep:
     # -- accounting ----------------------------------------------------------
     def launches(self) -> int:
         """Kernels one run() launches (centre scoring + selection, or the five
-        operators; + the gather)."""
-        return (2 if self.fused_select else 5) + (1 if self.gather else 0)
+        operators; + the gather; + the attention)."""
+        return (2 if self.fused_select else 5) + (1 if self.gather else 0) + (1 if self.attention is not None else 0)
 
     def algorithmic_bytes(self) -> dict:
         """Compulsory bytes of one step, each input byte once, each output once

@@ -633,6 +633,70 @@ V1X_API int v1x_gather_slots(const void* k, const void* v, const int32_t* req, c
                      int64_t ids_stride, int64_t dim, int64_t elem_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Extension: latent attention, absorbed form (no reference counterpart; the
+ * reference hands the selected rows to an external attention, NA/backend.py:9).
+ *   s[h, j] = scale * q[r, h, :] . pool[slot_j, :];  out[r, h, :] = sum_j
+ *   softmax_j(s[h, :]) pool[slot_j, 0:latent];  lse[r, h] = ln sum_j exp(s[h, j])
+ * over the tokens j of row r, j < count:
+ *   lens == NULL: slot_j = index[r, j] (or req[index[r, j]] with req, an i32 array
+ *     of req_len entries); an id < 0 or >= req_len is no token;
+ *   lens != NULL: j < min(lens[r], count), slot_j = index[r, j / 64] * 64 + j % 64
+ *     (index: page table of count / 64 columns; req NULL);
+ * a slot outside [0, slots) is no token.  A row without tokens: out 0, lse -inf.
+ * q [rows, heads, dim] with strides qs0, qs1; pool [slots, dim] with row stride
+ * pool_stride; out [rows, heads, latent] contiguous; dtype of q, pool and out: 1
+ * bf16, 2 f16; every address and stride a multiple of 16 bytes.  latent in {128,
+ * 256, 384, 512}, dim - latent in {0, 64}, heads <= 1024.  workspace: device
+ * memory of at least v1x_latent_attention_workspace(...) bytes, 16-byte aligned,
+ * of no meaning before or after the call (NULL if 0 bytes).  status: optional
+ * device word for V1X_STATUS_TIMEOUT. */
+V1X_API int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, int64_t count, int64_t latent);
+V1X_API int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, const void* pool, int64_t slots,
+                  int64_t pool_stride, const int32_t* req, int64_t req_len, const int32_t* index,
+                  int64_t index_stride, int64_t count, const int32_t* lens, int64_t rows, int64_t heads,
+                  int64_t dim, int64_t latent, float scale, int dtype, void* out, float* lse, void* workspace,
+                  int64_t workspace_bytes, int32_t* status, void* stream);
+
+/* Extension: latent attention, expanded form, for ragged prompts.  Request r has
+ * the queries offsets[r] .. offsets[r+1] and the keys kv_offsets[r] ..
+ * kv_offsets[r+1] (i32, non-decreasing; clamped to [0, tokens] / [0, keys]); its
+ * i-th query of nq sees the first i + 1 + nk - nq keys of its nk:
+ *   s[i, j] = scale * (q[i, h, 0:128] . k[j, h, :] + q[i, h, 128:128+dr] . k_rope[j, :])
+ * out [tokens, heads, 128] and lse [tokens, heads], contiguous; rows of no request
+ * are not written.  dr 0 (k_rope NULL) or 64; k, v rows of 128.  Types, alignment
+ * and status as above. */
+V1X_API int v1x_prompt_attention(const void* q, int64_t qs0, int64_t qs1, const void* k, int64_t ks0, int64_t ks1,
+                  const void* k_rope, int64_t krs0, const void* v, int64_t vs0, int64_t vs1,
+                  const int32_t* offsets, const int32_t* kv_offsets, int64_t requests, int64_t tokens,
+                  int64_t keys, int64_t heads, int64_t dr, float scale, int dtype, void* out, float* lse,
+                  int32_t* status, void* stream);
+
+/* Extension: a paged K/V cache in 8 bits.  Codes e4m3 [pages, heads, 64, 128] and
+ * power-of-two scales f32 [pages, heads] for K and V, contiguous, 16-byte aligned.
+ * store: the rows offsets[r] .. offsets[r+1] of k, v [tokens, heads, 128] (strides
+ * ks0, ks1 / vs0, vs1; dtype 1 bf16, 2 f16) become the tokens prefix[r], ... of
+ * request r, token t in page table[r, t / 64].  A page's scale is the smallest 2^e,
+ * -40 <= e <= 40, with 448 * 2^e >= the magnitudes stored, and does not fall below
+ * the page's former scale if it holds earlier tokens, whose codes are rounded again
+ * where it rises.  Tokens past the table or in a page outside the cache are dropped;
+ * places behind the last token are not written. */
+V1X_API int v1x_kv8_store(uint8_t* k_cache, float* k_scale, uint8_t* v_cache, float* v_scale, int64_t pages,
+                  int64_t heads, const void* k, int64_t ks0, int64_t ks1, const void* v, int64_t vs0, int64_t vs1,
+                  int dtype, int64_t tokens, const int32_t* table, int64_t table_stride, int64_t table_pages,
+                  const int32_t* prefix, const int32_t* offsets, int64_t requests, void* stream);
+
+/* Softmax attention of q [rows, heads, 128] over the first min(lens[r], 64 *
+ * table_pages) tokens of row r in that cache, heads / kv_heads query heads per K/V
+ * head; out [rows, heads, 128] in q's type and lse [rows, heads] contiguous.  A page
+ * outside the cache holds no tokens.  workspace as in v1x_latent_attention. */
+V1X_API int64_t v1x_kv8_attend_workspace(int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_pages);
+V1X_API int v1x_kv8_attend(const void* q, int64_t qs0, int64_t qs1, const uint8_t* k_cache, const float* k_scale,
+                  const uint8_t* v_cache, const float* v_scale, int64_t pages, int64_t kv_heads,
+                  const int32_t* table, int64_t table_stride, int64_t table_pages, const int32_t* lens,
+                  int64_t rows, int64_t heads, float scale, int dtype, void* out, float* lse, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Extension (no reference counterpart): failure-detection self test.  Launches
  * one kernel that waits, with the same bounded mbarrier wait the pipelined
  * kernels use, on a barrier nothing arrives at; after limit_ns (plus at most
