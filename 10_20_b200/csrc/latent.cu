@@ -1,14 +1,57 @@
-// Latent attention, absorbed form: see v1x_latent_attention in v1x.h.
+// Latent attention, absorbed form, on the tensor cores: see v1x_latent_attention
+// in v1x.h.
 //
-// One warp per (row, head): the query in registers, one token per step, the
-// running maximum and sum of the softmax (in powers of two) and the output row
-// in registers; one pass over the tokens.
+// Every head reads the same rows, as keys (all of a row) and as values (its first
+// `latent` elements), so a tile of 64 tokens is brought into shared memory once
+// and is an operand of both products:
+//
+//   S[64 heads x 64 tokens]      = Q . K^T        M = 64, N = 64, K = dim
+//   O^T[128 of latent x heads]  += V^T . P^T      M = 128, N = heads, K = 64
+//
+// S has one head per TMEM lane, so a head's softmax is one thread's work; the
+// output is kept transposed because its M is then the latent width, full 128-row
+// operands for any number of heads, and four accumulators of 64 columns leave
+// room for two score tiles.  The same bytes serve as K-major (keys) and MN-major
+// (values) operand.  Softmax in one pass, in powers of two: the running maximum
+// that the weights are taken against moves only when a tile exceeds it by more
+// than 2^8, so that O is rescaled a few times a row at most; sums stay in 32
+// bits, the weights are rounded once, to the inputs' type, for the second product.
+//
+// Work: the 64-token tiles of all rows in a line, cut into equal ranges, one CTA
+// each (times the groups of 64 heads, neighbours in the grid, which read the same
+// tiles at the same time from L2).  A row that lies in several ranges leaves
+// unnormalised parts in the workspace, joined by latent_join_kernel in the order
+// of the ranges.
+//
+// Warp roles (448 threads, one CTA per SM):
+//   0-3   softmax, rescale, epilogue (TMEM lane quarters 0-3)
+//   4-11  two groups of producers, alternate tiles: rows by 16-byte cp.async into
+//         the swizzled layout, each row's slot looked up a tile ahead; a token
+//         that is none becomes zeros and a cleared bit of the tile's mask
+//   12    TMEM owner, MMA issuer (one thread): the next tile's S and the current
+//         tile's O, whichever is ready
+//   13    the queries, when the row changes
+// Waits are bounded (2 s, then V1X_STATUS_TIMEOUT).
+#include <type_traits>
+
 #include "attention.cuh"
+#include "sm100.cuh"
 
 namespace v1x {
 namespace {
 
 using namespace attn;
+using namespace sm100;
+
+constexpr int kTile = 64;                // tokens of a tile
+constexpr int kGroup = 64;               // heads of a CTA
+constexpr int kBlock = 64 * 128;         // bytes of a 64 x 64 operand block
+constexpr int kMaxStages = 6;
+constexpr int kThreads = 448;
+constexpr int kMaxCtas = 148;
+constexpr uint32_t kScoreCol = 256;      // TMEM: O^T in columns 0-255, two score tiles after it
+constexpr float kLazy = 8.0f;            // log2 of the growth that the weights may show before a rescale
+constexpr uint64_t kWaitNs = 2000000000ull;
 
 struct LatentArgs {
   const void* q;
@@ -21,15 +64,50 @@ struct LatentArgs {
   int64_t index_stride, count;
   const int32_t* lens;
   int64_t rows, heads;
-  int dim, latent;
+  int chunks, latent, stages, groups, ranges;
   float scale_log2;
   void* out;
   float* lse;
+  float* part;       // [ranges * groups][2][64][latent], then [..][2][64][2] maxima and sums
+  float* part_ml;
+  int64_t* where;    // [ranges][4]: the row, its first tile in the line, its tiles, all tiles
+  int32_t* status;
+};
+
+struct LatentShared {
+  uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full, pv_done, q_full, q_empty;
+  uint64_t mask[kMaxStages];
+  float factor[kGroup];
+  int64_t start[4];  // as LatentArgs::where
+  int64_t scan[kThreads / 32 + 1];
+  uint32_t tmem;
+  int abort, zero;
+};
+
+__device__ __forceinline__ int64_t row_len(const LatentArgs& a, int64_t r) {
+  return a.lens ? min(static_cast<int64_t>(max(a.lens[r], 0)), a.count) : a.count;
+}
+__device__ __forceinline__ int64_t row_tiles(const LatentArgs& a, int64_t r) { return (row_len(a, r) + kTile - 1) / kTile; }
+
+// A place in the line of tiles.
+struct Place {
+  int64_t row, tile, tiles;  // the row, the tile of the row, the row's tiles
+  __device__ bool first() const { return tile == 0; }
+  __device__ bool last() const { return tile == tiles - 1; }
+  __device__ void next(const LatentArgs& a) {
+    if (++tile < tiles) return;
+    tile = 0;
+    do {
+      ++row;
+      tiles = row < a.rows ? row_tiles(a, row) : 1;
+    } while (tiles == 0);
+  }
 };
 
 // The pool slot of token j of row r, or -1 if there is none.
-__device__ __forceinline__ int64_t slot_of(const LatentArgs& a, const int32_t* index, int64_t j, int64_t n) {
-  if (j >= n) return -1;
+__device__ __forceinline__ int64_t slot_of(const LatentArgs& a, int64_t r, int64_t j) {
+  if (j >= row_len(a, r)) return -1;
+  const int32_t* index = a.index + r * a.index_stride;
   int64_t s;
   if (a.lens) {
     s = static_cast<int64_t>(index[j >> 6]) * 64 + (j & 63);
@@ -40,61 +118,455 @@ __device__ __forceinline__ int64_t slot_of(const LatentArgs& a, const int32_t* i
   return s >= 0 && s < a.slots ? s : -1;
 }
 
-constexpr int kMaxPairs = 9;  // 576 = 32 lanes * 9 pairs
+__device__ __forceinline__ int64_t range_start(int64_t tiles, int64_t x, int64_t ranges) { return tiles * x / ranges; }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void give_up(LatentShared& sh, int32_t* status) {
+  *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+  if (status) atomicExch(status, V1X_STATUS_TIMEOUT);
+}
+
+__device__ __forceinline__ bool any_of_128(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(x))
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void sync_128() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+
+// Rows of `chunks` 64-element blocks into the swizzled operand layout: row R (of
+// 64) of block c at c * kBlock + R * 128, its 16-byte pieces permuted by R & 7.
+// A group of eight lanes moves one 128-byte piece of a row at a time; the warp
+// covers the 16 rows R0 .. R0 + 15, whose sources `src` (per lane l < 16: row R0 + l,
+// null for zeros) are handed over by shuffles.
+__device__ __forceinline__ void copy_rows(uint32_t dst, const char* src, const void* any, int R0, int chunks, int lane) {
+  const char* from[4];
+  uint32_t to[4], bytes[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 4 * i + (lane >> 3), R = R0 + row;
+    const char* p = reinterpret_cast<const char*>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), row));
+    bytes[i] = p ? 16 : 0;
+    from[i] = p ? p + (lane & 7) * 16 : static_cast<const char*>(any);
+    to[i] = dst + R * 128 + (((lane & 7) ^ (R & 7)) << 4);
+  }
+#pragma unroll 3
+  for (int c = 0; c < chunks; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cp_async16(to[i] + c * kBlock, from[i] + (bytes[i] ? c * 128 : 0), bytes[i]);
+}
 
 template <typename T>
-__global__ void __launch_bounds__(128) latent_rows_kernel(const __grid_constant__ LatentArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t h = static_cast<int64_t>(blockIdx.y) * 4 + (threadIdx.x >> 5), r = blockIdx.x;
-  if (h >= a.heads) return;
-  const T* q = static_cast<const T*>(a.q) + r * a.qs0 + h * a.qs1;
-  const int32_t* index = a.index + r * a.index_stride;
-  const int64_t n = a.lens ? min(static_cast<int64_t>(max(a.lens[r], 0)), a.count) : a.count;
-  float2 qv[kMaxPairs], acc[kMaxPairs];
-#pragma unroll
-  for (int i = 0; i < kMaxPairs; ++i) {
-    const int d = 2 * (lane + 32 * i);
-    qv[i] = d < a.dim ? to_float2<T>(*reinterpret_cast<const uint32_t*>(q + d)) : make_float2(0.0f, 0.0f);
-    acc[i] = make_float2(0.0f, 0.0f);
-  }
-  float m = -CUDART_INF_F, l = 0.0f;
-  for (int64_t j = 0; j < n; ++j) {
-    const int64_t s = slot_of(a, index, j, n);
-    if (s < 0) continue;
-    const T* row = static_cast<const T*>(a.pool) + s * a.pool_stride;
-    float2 kv[kMaxPairs];
-    float dot = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kMaxPairs; ++i) {
-      const int d = 2 * (lane + 32 * i);
-      kv[i] = d < a.dim ? to_float2<T>(*reinterpret_cast<const uint32_t*>(row + d)) : make_float2(0.0f, 0.0f);
-      dot = fmaf(qv[i].x, kv[i].x, fmaf(qv[i].y, kv[i].y, dot));
+__global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_constant__ LatentArgs a) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t q_smem = smem_u32(base);
+  const uint32_t kv_smem = q_smem + a.chunks * kBlock;
+  uint8_t* p_ptr = base + (1 + a.stages) * a.chunks * kBlock;
+  const uint32_t p_smem = smem_u32(p_ptr);
+  LatentShared& sh = *reinterpret_cast<LatentShared*>(p_ptr + kBlock);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = blockIdx.x % a.groups;
+  const int64_t x = blockIdx.x / a.groups;
+  const int heads = min(kGroup, static_cast<int>(a.heads - group * kGroup));
+
+  if (tid == 0) {
+    sh.abort = 0;
+    sh.zero = 0;
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&sh.full[s], 128);
+      mbar_init(&sh.empty[s], 1);
     }
-    const float x = warp_sum(dot) * a.scale_log2, top = fmaxf(m, x);
-    const float shrink = exp2f(m - top), p = exp2f(x - top);
-    l = l * shrink + p;
-    m = top;
-#pragma unroll
-    for (int i = 0; i < kMaxPairs; ++i) {
-      acc[i].x = fmaf(p, kv[i].x, acc[i].x * shrink);
-      acc[i].y = fmaf(p, kv[i].y, acc[i].y * shrink);
+    mbar_init(&sh.s_full[0], 1);
+    mbar_init(&sh.s_full[1], 1);
+    mbar_init(&sh.p_full, 128);
+    mbar_init(&sh.pv_done, 1);
+    mbar_init(&sh.q_full, 32);
+    mbar_init(&sh.q_empty, 1);
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  // ---- this CTA's range of the line ---------------------------------------------
+  if (tid == 0) {
+    const int64_t per = a.lens ? 0 : (a.count + kTile - 1) / kTile, all = per * a.rows;
+    const int64_t row = per ? range_start(all, x, a.ranges) / per : 0;
+    sh.start[0] = row;
+    sh.start[1] = row * per;
+    sh.start[2] = per ? per : 1;
+    sh.start[3] = all;
+  }
+  __syncthreads();
+  if (a.lens) {
+    const int64_t chunk = (a.rows + kThreads - 1) / kThreads;
+    const int64_t beg = min(tid * chunk, a.rows), end = min(beg + chunk, a.rows);
+    int64_t mine = 0, all;
+    for (int64_t r = beg; r < end; ++r) mine += row_tiles(a, r);
+    int64_t run = block_exclusive_scan(mine, sh.scan, &all);
+    const int64_t t0 = range_start(all, x, a.ranges);
+    if (tid == 0) sh.start[3] = all;
+    if (run <= t0 && t0 < run + mine) {
+      for (int64_t r = beg; r < end; ++r) {
+        const int64_t n = row_tiles(a, r);
+        if (t0 < run + n) {
+          sh.start[0] = r;
+          sh.start[1] = run;
+          sh.start[2] = n;
+          break;
+        }
+        run += n;
+      }
     }
+    __syncthreads();
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  T* out = static_cast<T*>(a.out) + (r * a.heads + h) * a.latent;
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int64_t t0 = range_start(sh.start[3], x, a.ranges);
+  const int64_t n = range_start(sh.start[3], x + 1, a.ranges) - t0;   // tiles of the range
+  Place at{sh.start[0], t0 - sh.start[1], sh.start[2]};
+  if (tid == 0 && group == 0 && a.where)
+    for (int i = 0; i < 4; ++i) a.where[4 * x + i] = sh.start[i];
+
+  if (warp < 4) {
+    // ---------------- softmax, rescale, epilogue ----------------
+    const int h = 16 * warp + lane;              // lanes 16-31 carry no head (M = 64 fills half a quarter)
+    const bool mine = lane < 16;
+    const uint32_t quarter = static_cast<uint32_t>(warp * 32) << 16;
+    const int cols = (heads + 31) & ~31;         // accumulator columns moved, 32 at a time
+    float m = -CUDART_INF_F, l = 0.0f;
+    bool fresh = true;                           // the tile begins a segment: tiles of one row in this range
+    int64_t segment = 0, segment_tile = 0;
+    // after a wait that gave up the loop goes on without waiting, so that all
+    // four warps still meet at their barriers
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int64_t phase) {
+      if (ok && !mbar_wait(bar, phase & 1, &sh.abort, kWaitNs)) {
+        give_up(sh, a.status);
+        ok = false;
+      }
+    };
+    for (int64_t it = 0; it < n; ++it) {
+      const int stage = static_cast<int>(it % a.stages);
+      wait(&sh.s_full[it & 1], it >> 1);
+      wait(&sh.full[stage], it / a.stages);      // complete already: the producers' mask
+      tc_fence_after();
+      uint32_t raw[2][32];
+      tmem_ld32(tmem + quarter + kScoreCol + (it & 1) * 64, raw[0]);
+      tmem_ld32(tmem + quarter + kScoreCol + (it & 1) * 64 + 32, raw[1]);
+      tmem_ld_wait();
+      const uint64_t valid = *reinterpret_cast<volatile uint64_t*>(&sh.mask[stage]);
+      float s[64];
 #pragma unroll
-  for (int i = 0; i < kMaxPairs; ++i) {
-    const int d = 2 * (lane + 32 * i);
-    if (d < a.latent) *reinterpret_cast<uint32_t*>(out + d) = pack2<T>(acc[i].x * inv, acc[i].y * inv);
+      for (int j = 0; j < 64; ++j) s[j] = __uint_as_float(raw[j >> 5][j & 31]) * a.scale_log2;
+      if (valid != ~0ull) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+          if (!((valid >> j) & 1)) s[j] = -CUDART_INF_F;
+      }
+      float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int j = 4; j < 64; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
+      const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if (fresh) {
+        m = most;
+        l = 0.0f;
+        segment_tile = at.tile;
+      } else {
+        const bool grows = mine && most > m + kLazy;
+        if (any_of_128(grows)) {
+          const float f = grows ? exp2_fast(m - most) : 1.0f;
+          if (grows) m = most;
+          l *= f;
+          if (mine) sh.factor[h] = f;
+          wait(&sh.pv_done, it - 1);
+          sync_128();
+          tc_fence_after();
+          for (int t = 0; t < a.latent / 128; ++t)
+            for (int c = 0; c < cols; c += 32) {
+              const uint32_t addr = tmem + quarter + t * 64 + c;
+              uint32_t o[32];
+              tmem_ld32(addr, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * sh.factor[c + j]);
+              tmem_st32(addr, o);
+            }
+          tmem_st_wait();
+        }
+      }
+      fresh = false;
+      const float ref = m == -CUDART_INF_F ? 0.0f : m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < 64; ++j) {
+        s[j] = exp2_fast(s[j] - ref);
+        sum[j & 3] += s[j];
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      // the weights' buffer is free once the previous tile's product has read it
+      if (it > 0) wait(&sh.pv_done, it - 1);
+      if (mine) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint4 v = make_uint4(pack2<T>(s[8 * c], s[8 * c + 1]), pack2<T>(s[8 * c + 2], s[8 * c + 3]),
+                               pack2<T>(s[8 * c + 4], s[8 * c + 5]), pack2<T>(s[8 * c + 6], s[8 * c + 7]));
+          *reinterpret_cast<uint4*>(p_ptr + h * 128 + ((c ^ (h & 7)) << 4)) = v;
+        }
+      }
+      fence_async_shared();
+      tc_fence_before();
+      mbar_arrive(&sh.p_full);
+
+      if (at.last() || it == n - 1) {
+        wait(&sh.pv_done, it);
+        tc_fence_after();
+        const bool whole = at.last() && segment_tile == 0;   // all of the row's tiles were here
+        const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (segment > 0 ? 1 : 0));
+        float* part = a.part + slot * kGroup * a.latent;
+        if (mine) {
+          const int64_t o = at.row * a.heads + group * kGroup + h;
+          if (whole) {
+            sh.factor[h] = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+            if (h < heads) a.lse[o] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
+          } else if (h < heads) {
+            a.part_ml[(slot * kGroup + h) * 2] = m;
+            a.part_ml[(slot * kGroup + h) * 2 + 1] = l;
+          }
+        }
+        sync_128();
+        for (int t = 0; t < a.latent / 128; ++t)
+          for (int c = 0; c < cols; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(tmem + quarter + t * 64 + c, o);
+            tmem_ld_wait();
+            const int d = t * 128 + warp * 32 + lane;
+            if (whole) {
+              T* out = static_cast<T*>(a.out) + (at.row * a.heads + group * kGroup) * a.latent + (d & ~1);
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {   // lane pairs exchange, so that a lane has two neighbours of one head
+                const float u = __uint_as_float(o[j]) * sh.factor[c + j];
+                const float v = __uint_as_float(o[j + 1]) * sh.factor[c + j + 1];
+                const float y = __shfl_xor_sync(0xffffffffu, lane & 1 ? u : v, 1);
+                const int hh = c + j + (lane & 1);
+                if (hh < heads)
+                  *reinterpret_cast<uint32_t*>(out + static_cast<int64_t>(hh) * a.latent) =
+                      lane & 1 ? pack2<T>(y, v) : pack2<T>(u, y);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (c + j < heads) part[static_cast<int64_t>(c + j) * a.latent + d] = __uint_as_float(o[j]);
+            }
+          }
+        tc_fence_before();
+        sync_128();                              // factor is free again
+        ++segment;
+        fresh = true;
+      }
+      at.next(a);
+    }
+    // rows that have no tile
+    if (a.lens || a.count == 0) {
+      for (int64_t r = x; r < a.rows; r += a.ranges) {
+        if (row_len(a, r) > 0) continue;
+        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (r * a.heads + group * kGroup) * a.latent);
+        for (int i = tid; i < heads * a.latent / 8; i += 128) out[i] = make_uint4(0, 0, 0, 0);
+        if (tid < heads) a.lse[r * a.heads + group * kGroup + tid] = -CUDART_INF_F;
+      }
+    }
+  } else if (warp < 12) {
+    // ---------------- producers ----------------
+    const int set = (warp - 4) >> 2, w = warp & 3;
+    for (int i = 0; i < set && i < n; ++i) at.next(a);
+    int64_t slot = set < n && lane < 16 ? slot_of(a, at.row, at.tile * kTile + 16 * w + lane) : -1;
+    for (int64_t it = set; it < n; it += 2) {
+      const int s = static_cast<int>(it % a.stages);
+      if (!mbar_wait(&sh.empty[s], ((it / a.stages) & 1) ^ 1, &sh.abort, kWaitNs)) {
+        give_up(sh, a.status);
+        break;
+      }
+      const unsigned some = __ballot_sync(0xffffffffu, slot >= 0) & 0xFFFFu;
+      if (lane == 0) reinterpret_cast<volatile uint16_t*>(&sh.mask[s])[w] = static_cast<uint16_t>(some);
+      const char* src = slot >= 0 ? static_cast<const char*>(a.pool) + slot * a.pool_stride * 2 : nullptr;
+      copy_rows(kv_smem + s * a.chunks * kBlock, src, a.q, 16 * w, a.chunks, lane);
+      if (it + 2 < n) {   // the next tile's slots arrive while this one's rows do
+        at.next(a);
+        at.next(a);
+        slot = lane < 16 ? slot_of(a, at.row, at.tile * kTile + 16 * w + lane) : -1;
+      }
+      cp_async_wait_all();
+      fence_async_shared();
+      mbar_arrive(&sh.full[s]);
+    }
+    cp_async_wait_all();
+  } else if (warp == 12) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0 && n > 0) {
+      const uint32_t qk = idesc_16bit_f32(kBf16, 64, 64, false, false);
+      const uint32_t pv = idesc_16bit_f32(kBf16, 128, (heads + 15) & ~15, true, false);
+      Place ahead = at;                          // the tile whose scores are issued next
+      int64_t scored = 0, done = 0, rows_scored = 0;
+      uint64_t t_idle = 0;
+      uint32_t spins = 0;
+      while (done < n) {
+        bool moved = false;
+        if (scored < n && scored <= done + 1) {
+          const int s = static_cast<int>(scored % a.stages);
+          const bool fresh = scored == 0 || ahead.first();
+          if (mbar_test(&sh.full[s], (scored / a.stages) & 1) && (!fresh || mbar_test(&sh.q_full, rows_scored & 1))) {
+            tc_fence_after();
+            const uint32_t kv = kv_smem + s * a.chunks * kBlock, d = tmem + kScoreCol + (scored & 1) * 64;
+            for (int c = 0; c < a.chunks; ++c)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16(d, umma_desc_sw128(q_smem + c * kBlock + 32 * k), umma_desc_sw128(kv + c * kBlock + 32 * k), qk,
+                         c + k > 0 ? 1u : 0u);
+            umma_commit(&sh.s_full[scored & 1]);
+            if (fresh) ++rows_scored;
+            if (ahead.last()) umma_commit(&sh.q_empty);
+            ahead.next(a);
+            ++scored;
+            moved = true;
+          }
+        }
+        if (done < scored && mbar_test(&sh.p_full, done & 1)) {
+          tc_fence_after();
+          const int s = static_cast<int>(done % a.stages);
+          const uint32_t kv = kv_smem + s * a.chunks * kBlock;
+          const uint32_t more = done == 0 || at.first() ? 0u : 1u;
+          for (int t = 0; t < a.latent / 128; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f16(tmem + t * 64, umma_desc_mn_sw128(kv + 2 * t * kBlock + 2048 * k, kBlock),
+                       umma_desc_sw128(p_smem + 32 * k), pv, k > 0 ? 1u : more);
+          umma_commit(&sh.empty[s]);
+          umma_commit(&sh.pv_done);
+          at.next(a);
+          ++done;
+          moved = true;
+        }
+        if (moved) {
+          t_idle = 0;
+        } else if ((++spins & 63) == 0) {
+          if (*reinterpret_cast<volatile int*>(&sh.abort)) break;
+          const uint64_t t = globaltimer_ns();
+          if (!t_idle) t_idle = t;
+          if (t - t_idle > kWaitNs) {
+            give_up(sh, a.status);
+            break;
+          }
+        }
+      }
+      // everything that was issued retires before the CTA ends
+      if (scored > 0) mbar_wait(&sh.s_full[(scored - 1) & 1], ((scored - 1) >> 1) & 1, &sh.zero, kWaitNs);
+      if (done > 0) {
+        mbar_wait(&sh.empty[(done - 1) % a.stages], ((done - 1) / a.stages) & 1, &sh.zero, kWaitNs);
+        mbar_wait(&sh.pv_done, (done - 1) & 1, &sh.zero, kWaitNs);
+      }
+    }
+  } else {
+    // ---------------- queries ----------------
+    int64_t rows_loaded = 0;
+    for (int64_t it = 0; it < n;) {
+      if (!mbar_wait(&sh.q_empty, (rows_loaded & 1) ^ 1, &sh.abort, kWaitNs)) {
+        give_up(sh, a.status);
+        break;
+      }
+      const char* q = static_cast<const char*>(a.q) + (at.row * a.qs0 + group * kGroup * a.qs1) * 2;
+      for (int w = 0; w < 4; ++w) {
+        const int hh = 16 * w + lane;
+        copy_rows(q_smem, lane < 16 && hh < heads ? q + hh * a.qs1 * 2 : nullptr, a.q, 16 * w, a.chunks, lane);
+      }
+      cp_async_wait_all();
+      fence_async_shared();
+      mbar_arrive(&sh.q_full);
+      ++rows_loaded;
+      it += at.tiles - at.tile;
+      at.tile = at.tiles - 1;
+      at.next(a);
+    }
+    cp_async_wait_all();
   }
-  if (lane == 0) a.lse[r * a.heads + h] = l > 0.0f ? (m + log2f(l)) * kLn2 : -CUDART_INF_F;
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
 }
+
+// Joins the parts of the rows that lie in several ranges.  Block (x, h): the row
+// in which range x begins, if x is the first range to begin inside it; the parts
+// in the order of the ranges.  Range x's part is its first (slot 0) unless the
+// range begins in an earlier row.
+template <typename T>
+__global__ void __launch_bounds__(128) latent_join_kernel(const __grid_constant__ LatentArgs a) {
+  const int64_t x = blockIdx.x + 1, h = blockIdx.y;
+  const int64_t row = a.where[4 * x], first = a.where[4 * x + 1], tiles = a.where[4 * x + 2], all = a.where[4 * x + 3];
+  if (range_start(all, x, a.ranges) == first || range_start(all, x - 1, a.ranges) > first) return;
+  int64_t end = x;
+  while (end < a.ranges && range_start(all, end, a.ranges) < first + tiles) ++end;
+  const int group = static_cast<int>(h / kGroup), hg = static_cast<int>(h % kGroup);
+  auto slot = [&](int64_t y) {
+    return (y * a.groups + group) * 2 + (range_start(all, y, a.ranges) < first ? 1 : 0);
+  };
+  auto empty = [&](int64_t y) { return range_start(all, y, a.ranges) == range_start(all, y + 1, a.ranges); };
+  float m = -CUDART_INF_F;
+#pragma unroll 4
+  for (int64_t y = x - 1; y < end; ++y)
+    if (!empty(y)) m = fmaxf(m, a.part_ml[(slot(y) * kGroup + hg) * 2]);
+  const float ref = m == -CUDART_INF_F ? 0.0f : m;
+  const int d = 4 * threadIdx.x;
+  const bool mine = d < a.latent;
+  float4 o = make_float4(0, 0, 0, 0);
+  float l = 0.0f;
+#pragma unroll 4
+  for (int64_t y = x - 1; y < end; ++y) {
+    if (empty(y)) continue;
+    const int64_t p = slot(y) * kGroup + hg;
+    const float f = exp2f(a.part_ml[2 * p] - ref);
+    l += a.part_ml[2 * p + 1] * f;
+    if (mine) {
+      const float4 v = *reinterpret_cast<const float4*>(a.part + p * a.latent + d);
+      o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+    }
+  }
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+  if (mine)
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (row * a.heads + h) * a.latent + d) =
+        make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+  if (threadIdx.x == 0) a.lse[row * a.heads + h] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
+}
+
+int64_t ranges_for(int64_t rows, int64_t heads, int64_t count) {
+  const int64_t groups = (heads + kGroup - 1) / kGroup, tiles = rows * ((count + kTile - 1) / kTile);
+  const int64_t fit = kMaxCtas / groups;
+  return tiles < fit ? (tiles > 0 ? tiles : 1) : fit;
+}
+
+constexpr int64_t kMaxSmem = 232448;
 
 }  // namespace
 }  // namespace v1x
 
 extern "C" int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, int64_t count, int64_t latent) {
-  return 0;
+  using namespace v1x;
+  if (rows <= 0 || heads <= 0 || heads > 1024 || count <= 0 || latent <= 0) return 0;
+  const int64_t ranges = ranges_for(rows, heads, count), ctas = ranges * ((heads + kGroup - 1) / kGroup);
+  return ranges * 32 + ctas * 2 * kGroup * (latent + 2) * 4;
 }
 
 extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, const void* pool, int64_t slots,
@@ -107,7 +579,8 @@ extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, con
   using namespace v1x::attn;
   clear_error();
   V1X_CHECK_ARG(dtype == 1 || dtype == 2, "latent_attention: dtype must be 1 (bf16) or 2 (f16)");
-  V1X_CHECK_ARG(rows >= 0 && rows < (int64_t(1) << 31) && heads >= 1 && heads <= 1024 && count >= 0 && slots >= 0,
+  V1X_CHECK_ARG(rows >= 0 && rows < (int64_t(1) << 31) && heads >= 1 && heads <= 1024 && count >= 0 &&
+                    count < (int64_t(1) << 37) && slots >= 0,
                 "latent_attention: bad geometry");
   V1X_CHECK_ARG(latent >= 128 && latent <= 512 && latent % 128 == 0 && (dim == latent || dim == latent + 64),
                 "latent_attention: latent must be 128, 256, 384 or 512 and dim - latent 0 or 64");
@@ -117,12 +590,38 @@ extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, con
   V1X_CHECK_ARG(!lens || (count % 64 == 0 && !req), "latent_attention: a page table takes whole pages and no slot map");
   if (rows == 0) return V1X_OK;
   V1X_CHECK_ARG(q && out && lse && (index || count == 0) && (pool || slots == 0), "latent_attention: NULL argument");
-  LatentArgs a{q,    qs0,  qs1,  pool,  slots, pool_stride, req, req_len, index, index_stride, count,
-               lens, rows, heads, static_cast<int>(dim), static_cast<int>(latent), scale * kLog2e, out, lse};
-  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>((heads + 3) / 4));
+  const int64_t need = v1x_latent_attention_workspace(rows, heads, count, latent);
+  V1X_CHECK_ARG(workspace_bytes >= need && (workspace || need == 0) && aligned16(workspace),
+                "latent_attention: the workspace must be 16-byte aligned and hold %lld bytes", static_cast<long long>(need));
+  cudaStream_t s = as_stream(stream);
+  const int64_t groups = (heads + kGroup - 1) / kGroup, ranges = ranges_for(rows, heads, count);
+  LatentArgs a{q,    qs0,  qs1,   pool, slots, pool_stride, req, req_len, index, index_stride, count, lens, rows, heads,
+               static_cast<int>(dim / 64), static_cast<int>(latent), 0, static_cast<int>(groups),
+               static_cast<int>(ranges), scale * kLog2e, out, lse, nullptr, nullptr, nullptr, status};
+  if (need) {
+    a.where = static_cast<int64_t*>(workspace);
+    a.part = reinterpret_cast<float*>(a.where + 4 * ranges);
+    a.part_ml = a.part + ranges * groups * 2 * kGroup * latent;
+  }
+  const int64_t fixed = kBlock + 1024 + static_cast<int64_t>(sizeof(LatentShared)), tile = a.chunks * kBlock;
+  int64_t stages = (kMaxSmem - fixed - tile) / tile;
+  a.stages = static_cast<int>(stages > kMaxStages ? kMaxStages : stages & ~int64_t(1));
+  const size_t smem = static_cast<size_t>(fixed + (1 + a.stages) * tile);
+  static DeviceOnce once;
+  once.run([] {
+    cudaFuncSetAttribute(latent_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    cudaFuncSetAttribute(latent_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  });
+  const dim3 grid(static_cast<unsigned>(ranges * groups)), join(static_cast<unsigned>(ranges - 1), static_cast<unsigned>(heads));
   if (dtype == 1)
-    launch_kernel_prio(LaunchPriority::kDefault, latent_rows_kernel<__nv_bfloat16>, grid, dim3(128), 0, as_stream(stream), a);
+    launch_kernel_prio(LaunchPriority::kDefault, latent_kernel<__nv_bfloat16>, grid, dim3(kThreads), smem, s, a);
   else
-    launch_kernel_prio(LaunchPriority::kDefault, latent_rows_kernel<__half>, grid, dim3(128), 0, as_stream(stream), a);
+    launch_kernel_prio(LaunchPriority::kDefault, latent_kernel<__half>, grid, dim3(kThreads), smem, s, a);
+  if (ranges > 1) {
+    if (dtype == 1)
+      launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<__nv_bfloat16>, join, dim3(128), 0, s, a);
+    else
+      launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<__half>, join, dim3(128), 0, s, a);
+  }
   return launch_status("v1x_latent_attention");
 }

@@ -260,8 +260,8 @@ class SelectionStep:
     # -- accounting ----------------------------------------------------------
     def launches(self) -> int:
         """Kernels one run() launches (centre scoring + selection, or the five
-        operators; + the gather; + the attention)."""
-        return (2 if self.fused_select else 5) + (1 if self.gather else 0) + (1 if self.attention is not None else 0)
+        operators; + the gather; + the attention and its join)."""
+        return (2 if self.fused_select else 5) + (1 if self.gather else 0) + (2 if self.attention is not None else 0)
 
     def algorithmic_bytes(self) -> dict:
         """Compulsory bytes of one step, each input byte once, each output once
