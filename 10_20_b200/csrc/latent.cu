@@ -28,7 +28,7 @@
 //   4-11  two groups of producers, alternate tiles: rows by 16-byte cp.async into
 //         the swizzled layout, each row's slot looked up a tile ahead; a token
 //         that is none becomes zeros and a cleared bit of the tile's mask
-//   12    TMEM owner, MMA issuer (one thread): the next tile's S and the current
+//   12    TMEM owner, MMA issuer: the next tile's S and the current
 //         tile's O, whichever is ready
 //   13    the queries, when the row changes
 // Waits are bounded (2 s, then V1X_STATUS_TIMEOUT).
@@ -64,13 +64,14 @@ struct LatentArgs {
   int64_t index_stride, count;
   const int32_t* lens;
   int64_t rows, heads;
-  int chunks, latent, stages, groups, ranges;
+  int stages, groups, ranges;
   float scale_log2;
   void* out;
   float* lse;
   float* part;       // [ranges * groups][2][64][latent], then [..][2][64][2] maxima and sums
   float* part_ml;
-  int64_t* where;    // [ranges][4]: the row, its first tile in the line, its tiles, all tiles
+  int64_t* where;    // [ranges + 1][4]: where range x begins: the row, its first tile in the line, its
+                     // tiles, and the range's own first tile; [ranges][3]: the number of all tiles
   int32_t* status;
 };
 
@@ -91,7 +92,7 @@ __device__ __forceinline__ int64_t row_tiles(const LatentArgs& a, int64_t r) { r
 
 // A place in the line of tiles.
 struct Place {
-  int64_t row, tile, tiles;  // the row, the tile of the row, the row's tiles
+  int row, tile, tiles;  // the row, the tile of the row, the row's tiles
   __device__ bool first() const { return tile == 0; }
   __device__ bool last() const { return tile == tiles - 1; }
   __device__ void next(const LatentArgs& a) {
@@ -99,7 +100,7 @@ struct Place {
     tile = 0;
     do {
       ++row;
-      tiles = row < a.rows ? row_tiles(a, row) : 1;
+      tiles = row < a.rows ? static_cast<int>(row_tiles(a, row)) : 1;
     } while (tiles == 0);
   }
 };
@@ -147,8 +148,10 @@ __device__ __forceinline__ void sync_128() { asm volatile("barrier.cta.sync 1, 1
 // 64) of block c at c * kBlock + R * 128, its 16-byte pieces permuted by R & 7.
 // A group of eight lanes moves one 128-byte piece of a row at a time; the warp
 // covers the 16 rows R0 .. R0 + 15, whose sources `src` (per lane l < 16: row R0 + l,
-// null for zeros) are handed over by shuffles.
-__device__ __forceinline__ void copy_rows(uint32_t dst, const char* src, const void* any, int R0, int chunks, int lane) {
+// null for zeros, `any` then being an address that is not read) are handed over by
+// shuffles.
+template <int kChunks>
+__device__ __forceinline__ void copy_rows(uint32_t dst, const char* src, const void* any, int R0, int lane) {
   const char* from[4];
   uint32_t to[4], bytes[4];
 #pragma unroll
@@ -160,20 +163,21 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, const char* src, const v
     from[i] = p ? p + (lane & 7) * 16 : static_cast<const char*>(any);
     to[i] = dst + R * 128 + (((lane & 7) ^ (R & 7)) << 4);
   }
-#pragma unroll 3
-  for (int c = 0; c < chunks; ++c)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) cp_async16(to[i] + c * kBlock, from[i] + (bytes[i] ? c * 128 : 0), bytes[i]);
+  for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cp_async16(to[i] + c * kBlock, from[i] + c * 128, bytes[i]);
 }
 
-template <typename T>
+template <typename T, int kLatent, int kRope>
 __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_constant__ LatentArgs a) {
+  constexpr int kChunks = (kLatent + kRope) / 64, kOut = kLatent / 128;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t q_smem = smem_u32(base);
-  const uint32_t kv_smem = q_smem + a.chunks * kBlock;
-  uint8_t* p_ptr = base + (1 + a.stages) * a.chunks * kBlock;
+  const uint32_t kv_smem = q_smem + kChunks * kBlock;
+  uint8_t* p_ptr = base + (1 + a.stages) * kChunks * kBlock;
   const uint32_t p_smem = smem_u32(p_ptr);
   LatentShared& sh = *reinterpret_cast<LatentShared*>(p_ptr + kBlock);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -236,10 +240,13 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   const int64_t t0 = range_start(sh.start[3], x, a.ranges);
-  const int64_t n = range_start(sh.start[3], x + 1, a.ranges) - t0;   // tiles of the range
-  Place at{sh.start[0], t0 - sh.start[1], sh.start[2]};
-  if (tid == 0 && group == 0 && a.where)
-    for (int i = 0; i < 4; ++i) a.where[4 * x + i] = sh.start[i];
+  const int n = static_cast<int>(range_start(sh.start[3], x + 1, a.ranges) - t0);   // tiles of the range
+  Place at{static_cast<int>(sh.start[0]), static_cast<int>(t0 - sh.start[1]), static_cast<int>(sh.start[2])};
+  if (tid == 0 && group == 0 && a.where) {
+    for (int i = 0; i < 3; ++i) a.where[4 * x + i] = sh.start[i];
+    a.where[4 * x + 3] = t0;
+    if (x == a.ranges - 1) a.where[4 * x + 7] = sh.start[3];
+  }
 
   if (warp < 4) {
     // ---------------- softmax, rescale, epilogue ----------------
@@ -249,26 +256,29 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     const int cols = (heads + 31) & ~31;         // accumulator columns moved, 32 at a time
     float m = -CUDART_INF_F, l = 0.0f;
     bool fresh = true;                           // the tile begins a segment: tiles of one row in this range
-    int64_t segment = 0, segment_tile = 0;
+    int segment = 0, segment_tile = 0, stage = 0, turn = 0;
     // after a wait that gave up the loop goes on without waiting, so that all
     // four warps still meet at their barriers
     bool ok = true;
-    auto wait = [&](uint64_t* bar, int64_t phase) {
+    auto wait = [&](uint64_t* bar, int phase) {
       if (ok && !mbar_wait(bar, phase & 1, &sh.abort, kWaitNs)) {
         give_up(sh, a.status);
         ok = false;
       }
     };
-    for (int64_t it = 0; it < n; ++it) {
-      const int stage = static_cast<int>(it % a.stages);
+    for (int it = 0; it < n; ++it) {
       wait(&sh.s_full[it & 1], it >> 1);
-      wait(&sh.full[stage], it / a.stages);      // complete already: the producers' mask
+      wait(&sh.full[stage], turn);               // complete already: the producers' mask
       tc_fence_after();
       uint32_t raw[2][32];
       tmem_ld32(tmem + quarter + kScoreCol + (it & 1) * 64, raw[0]);
       tmem_ld32(tmem + quarter + kScoreCol + (it & 1) * 64 + 32, raw[1]);
       tmem_ld_wait();
       const uint64_t valid = *reinterpret_cast<volatile uint64_t*>(&sh.mask[stage]);
+      if (++stage == a.stages) {
+        stage = 0;
+        ++turn;
+      }
       float s[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) s[j] = __uint_as_float(raw[j >> 5][j & 31]) * a.scale_log2;
@@ -295,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
           wait(&sh.pv_done, it - 1);
           sync_128();
           tc_fence_after();
-          for (int t = 0; t < a.latent / 128; ++t)
+          for (int t = 0; t < kOut; ++t)
             for (int c = 0; c < cols; c += 32) {
               const uint32_t addr = tmem + quarter + t * 64 + c;
               uint32_t o[32];
@@ -336,9 +346,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
         tc_fence_after();
         const bool whole = at.last() && segment_tile == 0;   // all of the row's tiles were here
         const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (segment > 0 ? 1 : 0));
-        float* part = a.part + slot * kGroup * a.latent;
+        float* part = a.part + slot * kGroup * kLatent;
         if (mine) {
-          const int64_t o = at.row * a.heads + group * kGroup + h;
+          const int64_t o = static_cast<int64_t>(at.row) * a.heads + group * kGroup + h;
           if (whole) {
             sh.factor[h] = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
             if (h < heads) a.lse[o] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
@@ -348,28 +358,31 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
           }
         }
         sync_128();
-        for (int t = 0; t < a.latent / 128; ++t)
+        T* const out = static_cast<T*>(a.out) + (static_cast<int64_t>(at.row) * a.heads + group * kGroup) * kLatent;
+#pragma unroll 1
+        for (int t = 0; t < kOut; ++t)
+#pragma unroll 1
           for (int c = 0; c < cols; c += 32) {
             uint32_t o[32];
             tmem_ld32(tmem + quarter + t * 64 + c, o);
             tmem_ld_wait();
-            const int d = t * 128 + warp * 32 + lane;
+            const int d = t * 128 + warp * 32 + lane, left = heads - c;
             if (whole) {
-              T* out = static_cast<T*>(a.out) + (at.row * a.heads + group * kGroup) * a.latent + (d & ~1);
+              // lane pairs exchange, so that a lane has two neighbours of one head
+              T* const to = out + c * kLatent + (lane & 1) * kLatent + (d & ~1);
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) {   // lane pairs exchange, so that a lane has two neighbours of one head
+              for (int j = 0; j < 32; j += 2) {
                 const float u = __uint_as_float(o[j]) * sh.factor[c + j];
                 const float v = __uint_as_float(o[j + 1]) * sh.factor[c + j + 1];
                 const float y = __shfl_xor_sync(0xffffffffu, lane & 1 ? u : v, 1);
-                const int hh = c + j + (lane & 1);
-                if (hh < heads)
-                  *reinterpret_cast<uint32_t*>(out + static_cast<int64_t>(hh) * a.latent) =
-                      lane & 1 ? pack2<T>(y, v) : pack2<T>(u, y);
+                const uint32_t two = lane & 1 ? pack2<T>(y, v) : pack2<T>(u, y);
+                if (j + (lane & 1) < left) *reinterpret_cast<uint32_t*>(to + j * kLatent) = two;
               }
             } else {
+              float* const to = part + c * kLatent + d;
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (c + j < heads) part[static_cast<int64_t>(c + j) * a.latent + d] = __uint_as_float(o[j]);
+                if (j < left) to[j * kLatent] = __uint_as_float(o[j]);
             }
           }
         tc_fence_before();
@@ -383,105 +396,115 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     if (a.lens || a.count == 0) {
       for (int64_t r = x; r < a.rows; r += a.ranges) {
         if (row_len(a, r) > 0) continue;
-        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (r * a.heads + group * kGroup) * a.latent);
-        for (int i = tid; i < heads * a.latent / 8; i += 128) out[i] = make_uint4(0, 0, 0, 0);
+        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (r * a.heads + group * kGroup) * kLatent);
+        for (int i = tid; i < heads * kLatent / 8; i += 128) out[i] = make_uint4(0, 0, 0, 0);
         if (tid < heads) a.lse[r * a.heads + group * kGroup + tid] = -CUDART_INF_F;
       }
     }
   } else if (warp < 12) {
     // ---------------- producers ----------------
     const int set = (warp - 4) >> 2, w = warp & 3;
+    int s = set, turn = 0;                       // the number of stages is even
     for (int i = 0; i < set && i < n; ++i) at.next(a);
-    int64_t slot = set < n && lane < 16 ? slot_of(a, at.row, at.tile * kTile + 16 * w + lane) : -1;
-    for (int64_t it = set; it < n; it += 2) {
-      const int s = static_cast<int>(it % a.stages);
-      if (!mbar_wait(&sh.empty[s], ((it / a.stages) & 1) ^ 1, &sh.abort, kWaitNs)) {
+    int64_t slot = set < n && lane < 16 ? slot_of(a, at.row, at.tile * static_cast<int64_t>(kTile) + 16 * w + lane) : -1;
+    for (int it = set; it < n; it += 2) {
+      if (!mbar_wait(&sh.empty[s], (turn & 1) ^ 1, &sh.abort, kWaitNs)) {
         give_up(sh, a.status);
         break;
       }
       const unsigned some = __ballot_sync(0xffffffffu, slot >= 0) & 0xFFFFu;
       if (lane == 0) reinterpret_cast<volatile uint16_t*>(&sh.mask[s])[w] = static_cast<uint16_t>(some);
       const char* src = slot >= 0 ? static_cast<const char*>(a.pool) + slot * a.pool_stride * 2 : nullptr;
-      copy_rows(kv_smem + s * a.chunks * kBlock, src, a.q, 16 * w, a.chunks, lane);
+      copy_rows<kChunks>(kv_smem + s * kChunks * kBlock, src, a.q, 16 * w, lane);
       if (it + 2 < n) {   // the next tile's slots arrive while this one's rows do
         at.next(a);
         at.next(a);
-        slot = lane < 16 ? slot_of(a, at.row, at.tile * kTile + 16 * w + lane) : -1;
+        slot = lane < 16 ? slot_of(a, at.row, at.tile * static_cast<int64_t>(kTile) + 16 * w + lane) : -1;
       }
       cp_async_wait_all();
       fence_async_shared();
       mbar_arrive(&sh.full[s]);
+      s += 2;
+      if (s >= a.stages) {
+        s = set;
+        ++turn;
+      }
     }
     cp_async_wait_all();
   } else if (warp == 12) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
       const uint32_t qk = idesc_16bit_f32(kBf16, 64, 64, false, false);
       const uint32_t pv = idesc_16bit_f32(kBf16, 128, (heads + 15) & ~15, true, false);
+      const uint32_t q_desc = desc_k(q_smem), p_desc = desc_k(p_smem);
       Place ahead = at;                          // the tile whose scores are issued next
-      int64_t scored = 0, done = 0, rows_scored = 0;
+      int scored = 0, done = 0, rows_scored = 0;
+      int s_stage = 0, s_turn = 0, o_stage = 0;
       uint64_t t_idle = 0;
       uint32_t spins = 0;
       while (done < n) {
         bool moved = false;
         if (scored < n && scored <= done + 1) {
-          const int s = static_cast<int>(scored % a.stages);
           const bool fresh = scored == 0 || ahead.first();
-          if (mbar_test(&sh.full[s], (scored / a.stages) & 1) && (!fresh || mbar_test(&sh.q_full, rows_scored & 1))) {
+          if (__all_sync(0xffffffffu, mbar_test(&sh.full[s_stage], s_turn & 1) &&
+                                          (!fresh || mbar_test(&sh.q_full, rows_scored & 1)))) {
             tc_fence_after();
-            const uint32_t kv = kv_smem + s * a.chunks * kBlock, d = tmem + kScoreCol + (scored & 1) * 64;
-            for (int c = 0; c < a.chunks; ++c)
+            const uint32_t k_desc = desc_k(kv_smem + s_stage * kChunks * kBlock), d = tmem + kScoreCol + (scored & 1) * 64;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                umma_f16(d, umma_desc_sw128(q_smem + c * kBlock + 32 * k), umma_desc_sw128(kv + c * kBlock + 32 * k), qk,
-                         c + k > 0 ? 1u : 0u);
-            umma_commit(&sh.s_full[scored & 1]);
+                umma_f16(d, q_desc + (c * kBlock + 32 * k) / 16, k_desc + (c * kBlock + 32 * k) / 16, qk, c + k > 0 ? 1u : 0u);
+            umma_commit_elect(&sh.s_full[scored & 1]);
             if (fresh) ++rows_scored;
-            if (ahead.last()) umma_commit(&sh.q_empty);
+            if (ahead.last()) umma_commit_elect(&sh.q_empty);
             ahead.next(a);
+            if (++s_stage == a.stages) {
+              s_stage = 0;
+              ++s_turn;
+            }
             ++scored;
             moved = true;
           }
         }
-        if (done < scored && mbar_test(&sh.p_full, done & 1)) {
+        if (done < scored && __all_sync(0xffffffffu, mbar_test(&sh.p_full, done & 1))) {
           tc_fence_after();
-          const int s = static_cast<int>(done % a.stages);
-          const uint32_t kv = kv_smem + s * a.chunks * kBlock;
+          const uint32_t v_desc = desc_mn(kv_smem + o_stage * kChunks * kBlock, kBlock);
           const uint32_t more = done == 0 || at.first() ? 0u : 1u;
-          for (int t = 0; t < a.latent / 128; ++t)
+#pragma unroll
+          for (int t = 0; t < kOut; ++t)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f16(tmem + t * 64, umma_desc_mn_sw128(kv + 2 * t * kBlock + 2048 * k, kBlock),
-                       umma_desc_sw128(p_smem + 32 * k), pv, k > 0 ? 1u : more);
-          umma_commit(&sh.empty[s]);
-          umma_commit(&sh.pv_done);
+              umma_f16(tmem + t * 64, v_desc + (2 * t * kBlock + 2048 * k) / 16, p_desc + 32 * k / 16, pv, k > 0 ? 1u : more);
+          umma_commit_elect(&sh.empty[o_stage]);
+          umma_commit_elect(&sh.pv_done);
           at.next(a);
+          if (++o_stage == a.stages) o_stage = 0;
           ++done;
           moved = true;
         }
         if (moved) {
           t_idle = 0;
         } else if ((++spins & 63) == 0) {
-          if (*reinterpret_cast<volatile int*>(&sh.abort)) break;
           const uint64_t t = globaltimer_ns();
           if (!t_idle) t_idle = t;
-          if (t - t_idle > kWaitNs) {
-            give_up(sh, a.status);
-            break;
-          }
+          const bool late = t - t_idle > kWaitNs;
+          if (late) give_up(sh, a.status);
+          if (__any_sync(0xffffffffu, late || *reinterpret_cast<volatile int*>(&sh.abort))) break;
         }
       }
       // everything that was issued retires before the CTA ends
       if (scored > 0) mbar_wait(&sh.s_full[(scored - 1) & 1], ((scored - 1) >> 1) & 1, &sh.zero, kWaitNs);
       if (done > 0) {
-        mbar_wait(&sh.empty[(done - 1) % a.stages], ((done - 1) / a.stages) & 1, &sh.zero, kWaitNs);
+        const int last = done - 1;
+        mbar_wait(&sh.empty[last % a.stages], (last / a.stages) & 1, &sh.zero, kWaitNs);
         mbar_wait(&sh.pv_done, (done - 1) & 1, &sh.zero, kWaitNs);
       }
     }
   } else {
     // ---------------- queries ----------------
-    int64_t rows_loaded = 0;
-    for (int64_t it = 0; it < n;) {
+    int rows_loaded = 0;
+    for (int it = 0; it < n;) {
       if (!mbar_wait(&sh.q_empty, (rows_loaded & 1) ^ 1, &sh.abort, kWaitNs)) {
         give_up(sh, a.status);
         break;
@@ -489,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       const char* q = static_cast<const char*>(a.q) + (at.row * a.qs0 + group * kGroup * a.qs1) * 2;
       for (int w = 0; w < 4; ++w) {
         const int hh = 16 * w + lane;
-        copy_rows(q_smem, lane < 16 && hh < heads ? q + hh * a.qs1 * 2 : nullptr, a.q, 16 * w, a.chunks, lane);
+        copy_rows<kChunks>(q_smem, lane < 16 && hh < heads ? q + hh * a.qs1 * 2 : nullptr, a.q, 16 * w, lane);
       }
       cp_async_wait_all();
       fence_async_shared();
@@ -510,46 +533,73 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
 
 // Joins the parts of the rows that lie in several ranges.  Block (x, h): the row
 // in which range x begins, if x is the first range to begin inside it; the parts
-// in the order of the ranges.  Range x's part is its first (slot 0) unless the
-// range begins in an earlier row.
-template <typename T>
+// in the order of the ranges.  Range y's part is its first (slot 0) unless the
+// range begins in an earlier row (then its last, slot 1).
+template <typename T, int kLatent>
 __global__ void __launch_bounds__(128) latent_join_kernel(const __grid_constant__ LatentArgs a) {
-  const int64_t x = blockIdx.x + 1, h = blockIdx.y;
-  const int64_t row = a.where[4 * x], first = a.where[4 * x + 1], tiles = a.where[4 * x + 2], all = a.where[4 * x + 3];
-  if (range_start(all, x, a.ranges) == first || range_start(all, x - 1, a.ranges) > first) return;
-  int64_t end = x;
-  while (end < a.ranges && range_start(all, end, a.ranges) < first + tiles) ++end;
-  const int group = static_cast<int>(h / kGroup), hg = static_cast<int>(h % kGroup);
-  auto slot = [&](int64_t y) {
-    return (y * a.groups + group) * 2 + (range_start(all, y, a.ranges) < first ? 1 : 0);
-  };
-  auto empty = [&](int64_t y) { return range_start(all, y, a.ranges) == range_start(all, y + 1, a.ranges); };
-  float m = -CUDART_INF_F;
-#pragma unroll 4
-  for (int64_t y = x - 1; y < end; ++y)
-    if (!empty(y)) m = fmaxf(m, a.part_ml[(slot(y) * kGroup + hg) * 2]);
-  const float ref = m == -CUDART_INF_F ? 0.0f : m;
-  const int d = 4 * threadIdx.x;
-  const bool mine = d < a.latent;
-  float4 o = make_float4(0, 0, 0, 0);
-  float l = 0.0f;
-#pragma unroll 4
-  for (int64_t y = x - 1; y < end; ++y) {
-    if (empty(y)) continue;
-    const int64_t p = slot(y) * kGroup + hg;
-    const float f = exp2f(a.part_ml[2 * p] - ref);
-    l += a.part_ml[2 * p + 1] * f;
-    if (mine) {
-      const float4 v = *reinterpret_cast<const float4*>(a.part + p * a.latent + d);
-      o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
-    }
+  __shared__ float weight[kMaxCtas];
+  __shared__ float red[8];
+  const int x = blockIdx.x + 1, h = blockIdx.y, tid = threadIdx.x;
+  const int64_t first = a.where[4 * x + 1], begin = a.where[4 * x + 3], before = a.where[4 * x - 1];
+  if (begin == first || before > first) return;
+  const int64_t row = a.where[4 * x], end = first + a.where[4 * x + 2];
+  const int group = h / kGroup, hg = h % kGroup;
+  const int64_t base = ((static_cast<int64_t>(x - 1) * a.groups + group) * 2) * kGroup + hg;   // range x - 1, slot 0
+  const int64_t step = static_cast<int64_t>(a.groups) * 2 * kGroup;
+  const int64_t shift = before < first ? kGroup : 0;   // range x - 1 may begin in an earlier row
+  // the parts' weights 2^(m - M); 0 for a range without tiles
+  float m = -CUDART_INF_F, l = 0.0f;
+  int parts = 0;
+  for (int i = tid; i < a.ranges - (x - 1); i += 128) {
+    const int64_t t0 = a.where[4 * (x - 1 + i) + 3], t1 = a.where[4 * (x + i) + 3];
+    if (t0 >= end) break;
+    parts = i + 1;
+    if (t1 > t0) m = fmaxf(m, a.part_ml[2 * (base + i * step + (i == 0 ? shift : 0))]);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    parts = max(parts, __shfl_xor_sync(0xffffffffu, parts, o));
+  }
+  if ((tid & 31) == 0) {
+    red[tid >> 5] = m;
+    red[4 + (tid >> 5)] = __int_as_float(parts);
+  }
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  parts = max(max(__float_as_int(red[4]), __float_as_int(red[5])), max(__float_as_int(red[6]), __float_as_int(red[7])));
+  const float ref = m == -CUDART_INF_F ? 0.0f : m;
+  for (int i = tid; i < parts; i += 128) {
+    const int64_t t0 = a.where[4 * (x - 1 + i) + 3], t1 = a.where[4 * (x + i) + 3];
+    const float* ml = a.part_ml + 2 * (base + i * step + (i == 0 ? shift : 0));
+    const float w = t1 > t0 ? exp2f(ml[0] - ref) : 0.0f;
+    weight[i] = t1 > t0 ? w : -1.0f;
+    if (t1 > t0) l += ml[1] * w;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  __syncthreads();
+  if ((tid & 31) == 0) red[tid >> 5] = l;
+  __syncthreads();
+  l = (red[0] + red[1]) + (red[2] + red[3]);
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-  if (mine)
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (row * a.heads + h) * a.latent + d) =
+  if (4 * tid < kLatent) {
+    float4 o = make_float4(0, 0, 0, 0);
+    const float* p = a.part + base * kLatent + 4 * tid;
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) {
+      const float w = weight[i];
+      if (w < 0.0f) continue;
+      const float4 v = *reinterpret_cast<const float4*>(p + (i * step + (i == 0 ? shift : 0)) * kLatent);
+      o = make_float4(fmaf(v.x, w, o.x), fmaf(v.y, w, o.y), fmaf(v.z, w, o.z), fmaf(v.w, w, o.w));
+    }
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (row * a.heads + h) * kLatent + 4 * tid) =
         make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
-  if (threadIdx.x == 0) a.lse[row * a.heads + h] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
+  }
+  if (tid == 0) a.lse[row * a.heads + h] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
 }
+
+constexpr int64_t kMaxSmem = 232448;
 
 int64_t ranges_for(int64_t rows, int64_t heads, int64_t count) {
   const int64_t groups = (heads + kGroup - 1) / kGroup, tiles = rows * ((count + kTile - 1) / kTile);
@@ -557,7 +607,34 @@ int64_t ranges_for(int64_t rows, int64_t heads, int64_t count) {
   return tiles < fit ? (tiles > 0 ? tiles : 1) : fit;
 }
 
-constexpr int64_t kMaxSmem = 232448;
+// Launches the kernels of one element type and one pair of widths.
+template <typename T, int kLatent, int kRope>
+void launch(LatentArgs a, cudaStream_t s) {
+  constexpr int64_t kFixed = kBlock + 1024 + static_cast<int64_t>(sizeof(LatentShared));
+  constexpr int64_t kStage = (kLatent + kRope) / 64 * kBlock;
+  constexpr int64_t kFit = (kMaxSmem - kFixed) / kStage - 1;
+  constexpr int kStages = static_cast<int>(kFit > kMaxStages ? kMaxStages : kFit & ~int64_t(1));
+  static_assert(kStages >= 2, "two stages at least");
+  constexpr int64_t kSmem = kFixed + (1 + kStages) * kStage;
+  a.stages = kStages;
+  static DeviceOnce once;
+  once.run([] {
+    cudaFuncSetAttribute(latent_kernel<T, kLatent, kRope>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  });
+  launch_kernel_prio(LaunchPriority::kDefault, latent_kernel<T, kLatent, kRope>,
+                     dim3(static_cast<unsigned>(a.ranges * a.groups)), dim3(kThreads), kSmem, s, a);
+  if (a.ranges > 1)
+    launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<T, kLatent>,
+                       dim3(static_cast<unsigned>(a.ranges - 1), static_cast<unsigned>(a.heads)), dim3(128), 0, s, a);
+}
+
+template <typename T>
+void launch_widths(const LatentArgs& a, int64_t latent, int64_t rope, cudaStream_t s) {
+  if (latent == 512) rope ? launch<T, 512, 64>(a, s) : launch<T, 512, 0>(a, s);
+  else if (latent == 384) rope ? launch<T, 384, 64>(a, s) : launch<T, 384, 0>(a, s);
+  else if (latent == 256) rope ? launch<T, 256, 64>(a, s) : launch<T, 256, 0>(a, s);
+  else rope ? launch<T, 128, 64>(a, s) : launch<T, 128, 0>(a, s);
+}
 
 }  // namespace
 }  // namespace v1x
@@ -566,7 +643,7 @@ extern "C" int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, i
   using namespace v1x;
   if (rows <= 0 || heads <= 0 || heads > 1024 || count <= 0 || latent <= 0) return 0;
   const int64_t ranges = ranges_for(rows, heads, count), ctas = ranges * ((heads + kGroup - 1) / kGroup);
-  return ranges * 32 + ctas * 2 * kGroup * (latent + 2) * 4;
+  return (ranges + 1) * 32 + ctas * 2 * kGroup * (latent + 2) * 4;
 }
 
 extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, const void* pool, int64_t slots,
@@ -580,7 +657,7 @@ extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, con
   clear_error();
   V1X_CHECK_ARG(dtype == 1 || dtype == 2, "latent_attention: dtype must be 1 (bf16) or 2 (f16)");
   V1X_CHECK_ARG(rows >= 0 && rows < (int64_t(1) << 31) && heads >= 1 && heads <= 1024 && count >= 0 &&
-                    count < (int64_t(1) << 37) && slots >= 0,
+                    count < (int64_t(1) << 36) && slots >= 0,
                 "latent_attention: bad geometry");
   V1X_CHECK_ARG(latent >= 128 && latent <= 512 && latent % 128 == 0 && (dim == latent || dim == latent + 64),
                 "latent_attention: latent must be 128, 256, 384 or 512 and dim - latent 0 or 64");
@@ -596,32 +673,13 @@ extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, con
   cudaStream_t s = as_stream(stream);
   const int64_t groups = (heads + kGroup - 1) / kGroup, ranges = ranges_for(rows, heads, count);
   LatentArgs a{q,    qs0,  qs1,   pool, slots, pool_stride, req, req_len, index, index_stride, count, lens, rows, heads,
-               static_cast<int>(dim / 64), static_cast<int>(latent), 0, static_cast<int>(groups),
-               static_cast<int>(ranges), scale * kLog2e, out, lse, nullptr, nullptr, nullptr, status};
+               0, static_cast<int>(groups), static_cast<int>(ranges), scale * kLog2e, out, lse, nullptr, nullptr, nullptr, status};
   if (need) {
     a.where = static_cast<int64_t*>(workspace);
-    a.part = reinterpret_cast<float*>(a.where + 4 * ranges);
+    a.part = reinterpret_cast<float*>(a.where + 4 * (ranges + 1));
     a.part_ml = a.part + ranges * groups * 2 * kGroup * latent;
   }
-  const int64_t fixed = kBlock + 1024 + static_cast<int64_t>(sizeof(LatentShared)), tile = a.chunks * kBlock;
-  int64_t stages = (kMaxSmem - fixed - tile) / tile;
-  a.stages = static_cast<int>(stages > kMaxStages ? kMaxStages : stages & ~int64_t(1));
-  const size_t smem = static_cast<size_t>(fixed + (1 + a.stages) * tile);
-  static DeviceOnce once;
-  once.run([] {
-    cudaFuncSetAttribute(latent_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
-    cudaFuncSetAttribute(latent_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
-  });
-  const dim3 grid(static_cast<unsigned>(ranges * groups)), join(static_cast<unsigned>(ranges - 1), static_cast<unsigned>(heads));
-  if (dtype == 1)
-    launch_kernel_prio(LaunchPriority::kDefault, latent_kernel<__nv_bfloat16>, grid, dim3(kThreads), smem, s, a);
-  else
-    launch_kernel_prio(LaunchPriority::kDefault, latent_kernel<__half>, grid, dim3(kThreads), smem, s, a);
-  if (ranges > 1) {
-    if (dtype == 1)
-      launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<__nv_bfloat16>, join, dim3(128), 0, s, a);
-    else
-      launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<__half>, join, dim3(128), 0, s, a);
-  }
+  if (dtype == 1) launch_widths<__nv_bfloat16>(a, latent, dim - latent, s);
+  else launch_widths<__half>(a, latent, dim - latent, s);
   return launch_status("v1x_latent_attention");
 }
