@@ -2,35 +2,43 @@
 // in v1x.h.
 //
 // Every head reads the same rows, as keys (all of a row) and as values (its first
-// `latent` elements), so a tile of 64 tokens is brought into shared memory once
+// `latent` elements), so a tile of 32 tokens is brought into shared memory once
 // and is an operand of both products:
 //
-//   S[64 heads x 64 tokens]      = Q . K^T        M = 64, N = 64, K = dim
-//   O^T[128 of latent x heads]  += V^T . P^T      M = 128, N = heads, K = 64
+//   S[64 heads x 32 tokens]      = Q . K^T        M = 64, N = 32, K = dim
+//   O^T[128 of latent x heads]  += V^T . P^T      M = 128, N = heads, K = 32
 //
-// S has one head per TMEM lane, so a head's softmax is one thread's work; the
-// output is kept transposed because its M is then the latent width, full 128-row
-// operands for any number of heads, and four accumulators of 64 columns leave
-// room for two score tiles.  The same bytes serve as K-major (keys) and MN-major
-// (values) operand.  Softmax in one pass, in powers of two: the running maximum
-// that the weights are taken against moves only when a tile exceeds it by more
-// than 2^8, so that O is rescaled a few times a row at most; sums stay in 32
-// bits, the weights are rounded once, to the inputs' type, for the second product.
+// The output is kept transposed because its M is then the latent width, full
+// 128-row operands for any number of heads, and its four accumulators of 64
+// columns leave room for the score tiles.  The same bytes serve as K-major (keys)
+// and MN-major (values) operand.  Softmax in one pass, in powers of two: the
+// running maximum that the weights are taken against moves only when a tile
+// exceeds it by more than 2^8, so that O is rescaled a few times a row at most;
+// sums stay in 32 bits, the weights are rounded once, to the inputs' type, for the
+// second product.
 //
-// Work: the 64-token tiles of all rows in a line, cut into equal ranges, one CTA
-// each (times the groups of 64 heads, neighbours in the grid, which read the same
-// tiles at the same time from L2).  A row that lies in several ranges leaves
-// unnormalised parts in the workspace, joined by latent_join_kernel in the order
-// of the ranges.
+// What bounds it: 72 KB of queries leave room for 144 KB of tokens, and a stage is
+// held from its first load to its last product, a chain of latencies (load,
+// scores, softmax, product).  Four stages of 32 tokens turn around faster than two
+// of 64 (DECODE64 -> DECODE32 us on the decode batch), although N = 32 costs the
+// scores' product a quarter of its rate.
 //
-// Warp roles (448 threads, one CTA per SM):
+// Work: the tiles of all rows in a line, cut into equal ranges, one CTA each (times
+// the groups of 64 heads, neighbours in the grid, which read the same tiles at the
+// same time from L2).  A row that lies in several ranges leaves unnormalised parts
+// in the workspace, joined by latent_join_kernel in the order of the ranges.
+//
+// Warp roles (480 threads, one CTA per SM):
 //   0-3   softmax, rescale, epilogue (TMEM lane quarters 0-3)
-//   4-11  two groups of producers, alternate tiles: rows by 16-byte cp.async into
-//         the swizzled layout, each row's slot looked up a tile ahead; a token
-//         that is none becomes zeros and a cleared bit of the tile's mask
-//   12    TMEM owner, MMA issuer: the next tile's S and the current
-//         tile's O, whichever is ready
-//   13    the queries, when the row changes
+//   4-11  four sets of two producer warps, every fourth tile: rows by 16-byte
+//         cp.async into the swizzled layout, each row's slot looked up a tile
+//         ahead; a token that is none becomes zeros and a cleared bit of the
+//         tile's mask
+//   12    TMEM owner; issues the scores' MMAs, up to four tiles ahead
+//   13    issues the outputs' MMAs: an MMA of these shapes takes 24 to 48 cycles and few
+//         are queued, so that one warp's waits between the products would leave the
+//         tensor cores idle (ONEWARP -> TWOWARPS us on the decode batch)
+//   14    the queries, when the row changes
 // Waits are bounded (2 s, then V1X_STATUS_TIMEOUT).
 #include <type_traits>
 
@@ -43,11 +51,14 @@ namespace {
 using namespace attn;
 using namespace sm100;
 
-constexpr int kTile = 64;                // tokens of a tile
+constexpr int kTile = 32;                // tokens of a tile
 constexpr int kGroup = 64;               // heads of a CTA
-constexpr int kBlock = 64 * 128;         // bytes of a 64 x 64 operand block
-constexpr int kMaxStages = 6;
-constexpr int kThreads = 448;
+constexpr int kQBlock = kGroup * 128;    // bytes of 64 elements of a tile's rows: queries, ...
+constexpr int kBlock = kTile * 128;      // ... tokens
+constexpr int kPBytes = kGroup * 128;    // two tiles' weights side by side in 128-byte rows
+constexpr int kSets = 4;                 // producer sets, two warps each
+constexpr int kMaxStages = 8;
+constexpr int kThreads = 480;
 constexpr int kMaxCtas = 148;
 constexpr uint32_t kScoreCol = 256;      // TMEM: O^T in columns 0-255, two score tiles after it
 constexpr float kLazy = 8.0f;            // log2 of the growth that the weights may show before a rescale
@@ -76,8 +87,8 @@ struct LatentArgs {
 };
 
 struct LatentShared {
-  uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full, pv_done, q_full, q_empty;
-  uint64_t mask[kMaxStages];
+  uint64_t full[kMaxStages], empty[kMaxStages], s_full[4], p_full[4], pv_done[2], q_full, q_empty;
+  uint32_t mask[kMaxStages], flags[kMaxStages];   // flags: 1 the first tile of a segment, 2 the last of a row
   float factor[kGroup];
   int64_t start[4];  // as LatentArgs::where
   int64_t scan[kThreads / 32 + 1];
@@ -132,6 +143,14 @@ __device__ __forceinline__ void give_up(LatentShared& sh, int32_t* status) {
   if (status) atomicExch(status, V1X_STATUS_TIMEOUT);
 }
 
+// A whole warp waits, and agrees on the outcome.
+__device__ __forceinline__ bool converged_wait(LatentShared& sh, int32_t* status, uint64_t* bar, int phase) {
+  const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, &sh.abort, kWaitNs));
+  if (!ok) give_up(sh, status);
+  tc_fence_after();
+  return ok;
+}
+
 __device__ __forceinline__ bool any_of_128(bool x) {
   uint32_t r;
   asm volatile(
@@ -144,13 +163,13 @@ __device__ __forceinline__ bool any_of_128(bool x) {
 }
 __device__ __forceinline__ void sync_128() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
-// Rows of `chunks` 64-element blocks into the swizzled operand layout: row R (of
-// 64) of block c at c * kBlock + R * 128, its 16-byte pieces permuted by R & 7.
+// Rows of kChunks 64-element blocks into the swizzled operand layout: row R of
+// block c at c * kBytes + R * 128, its 16-byte pieces permuted by R & 7.
 // A group of eight lanes moves one 128-byte piece of a row at a time; the warp
 // covers the 16 rows R0 .. R0 + 15, whose sources `src` (per lane l < 16: row R0 + l,
 // null for zeros, `any` then being an address that is not read) are handed over by
 // shuffles.
-template <int kChunks>
+template <int kChunks, int kBytes>
 __device__ __forceinline__ void copy_rows(uint32_t dst, const char* src, const void* any, int R0, int lane) {
   const char* from[4];
   uint32_t to[4], bytes[4];
@@ -166,7 +185,7 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, const char* src, const v
 #pragma unroll
   for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) cp_async16(to[i] + c * kBlock, from[i] + c * 128, bytes[i]);
+    for (int i = 0; i < 4; ++i) cp_async16(to[i] + c * kBytes, from[i] + c * 128, bytes[i]);
 }
 
 template <typename T, int kLatent, int kRope>
@@ -176,10 +195,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t q_smem = smem_u32(base);
-  const uint32_t kv_smem = q_smem + kChunks * kBlock;
-  uint8_t* p_ptr = base + (1 + a.stages) * kChunks * kBlock;
+  const uint32_t kv_smem = q_smem + kChunks * kQBlock;
+  uint8_t* p_ptr = base + kChunks * (kQBlock + a.stages * kBlock);
   const uint32_t p_smem = smem_u32(p_ptr);
-  LatentShared& sh = *reinterpret_cast<LatentShared*>(p_ptr + kBlock);
+  LatentShared& sh = *reinterpret_cast<LatentShared*>(p_ptr + kPBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = blockIdx.x % a.groups;
   const int64_t x = blockIdx.x / a.groups;
@@ -189,14 +208,15 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     sh.abort = 0;
     sh.zero = 0;
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(&sh.full[s], 128);
+      mbar_init(&sh.full[s], 2);
       mbar_init(&sh.empty[s], 1);
     }
-    mbar_init(&sh.s_full[0], 1);
-    mbar_init(&sh.s_full[1], 1);
-    mbar_init(&sh.p_full, 128);
-    mbar_init(&sh.pv_done, 1);
-    mbar_init(&sh.q_full, 32);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.pv_done[i], 1);
+    mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1);
     fence_mbar_init();
   }
@@ -250,8 +270,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
 
   if (warp < 4) {
     // ---------------- softmax, rescale, epilogue ----------------
-    const int h = 16 * warp + lane;              // lanes 16-31 carry no head (M = 64 fills half a quarter)
-    const bool mine = lane < 16;
+    // M = 64 fills the lower half of each lane quarter: a head belongs to two
+    // threads, the even and the odd tokens of a tile
+    const int h = 16 * warp + (lane >> 2) + 8 * (lane & 1), odd = (lane >> 1) & 1;
+    const bool mine = odd == 0;                  // the one that speaks for the head
     const uint32_t quarter = static_cast<uint32_t>(warp * 32) << 16;
     const int cols = (heads + 31) & ~31;         // accumulator columns moved, 32 at a time
     float m = -CUDART_INF_F, l = 0.0f;
@@ -267,42 +289,42 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       }
     };
     for (int it = 0; it < n; ++it) {
-      wait(&sh.s_full[it & 1], it >> 1);
+      wait(&sh.s_full[it & 3], it >> 2);
       wait(&sh.full[stage], turn);               // complete already: the producers' mask
       tc_fence_after();
-      uint32_t raw[2][32];
-      tmem_ld32(tmem + quarter + kScoreCol + (it & 1) * 64, raw[0]);
-      tmem_ld32(tmem + quarter + kScoreCol + (it & 1) * 64 + 32, raw[1]);
-      tmem_ld_wait();
-      const uint64_t valid = *reinterpret_cast<volatile uint64_t*>(&sh.mask[stage]);
+      uint32_t raw[16];
+      tmem_ld16x32(tmem + quarter + kScoreCol + (it & 3) * kTile, raw);
+      const uint32_t valid = *reinterpret_cast<volatile uint32_t*>(&sh.mask[stage]);
       if (++stage == a.stages) {
         stage = 0;
         ++turn;
       }
-      float s[64];
+      tmem_ld_wait();
+      float s[16];
 #pragma unroll
-      for (int j = 0; j < 64; ++j) s[j] = __uint_as_float(raw[j >> 5][j & 31]) * a.scale_log2;
-      if (valid != ~0ull) {
+      for (int j = 0; j < 16; ++j) s[j] = __uint_as_float(raw[j]) * a.scale_log2;
+      if (valid != ~0u) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j)
-          if (!((valid >> j) & 1)) s[j] = -CUDART_INF_F;
+        for (int j = 0; j < 16; ++j)
+          if (!((valid >> (2 * j + odd)) & 1)) s[j] = -CUDART_INF_F;
       }
       float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int j = 4; j < 64; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
-      const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      for (int j = 4; j < 16; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
+      float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       if (fresh) {
         m = most;
         l = 0.0f;
         segment_tile = at.tile;
       } else {
-        const bool grows = mine && most > m + kLazy;
+        const bool grows = most > m + kLazy;
         if (any_of_128(grows)) {
           const float f = grows ? exp2_fast(m - most) : 1.0f;
           if (grows) m = most;
           l *= f;
           if (mine) sh.factor[h] = f;
-          wait(&sh.pv_done, it - 1);
+          wait(&sh.pv_done[(it - 1) & 1], (it - 1) >> 1);
           sync_128();
           tc_fence_after();
           for (int t = 0; t < kOut; ++t)
@@ -322,27 +344,33 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       const float ref = m == -CUDART_INF_F ? 0.0f : m;
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int j = 0; j < 64; ++j) {
+      for (int j = 0; j < 16; ++j) {
         s[j] = exp2_fast(s[j] - ref);
         sum[j & 3] += s[j];
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      // the weights' buffer is free once the previous tile's product has read it
-      if (it > 0) wait(&sh.pv_done, it - 1);
-      if (mine) {
+      // neighbouring tokens' weights meet in one thread: tokens 0-15 of the tile in
+      // the even one, 16-31 in the odd one
+      uint32_t w[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint4 v = make_uint4(pack2<T>(s[8 * c], s[8 * c + 1]), pack2<T>(s[8 * c + 2], s[8 * c + 3]),
-                               pack2<T>(s[8 * c + 4], s[8 * c + 5]), pack2<T>(s[8 * c + 6], s[8 * c + 7]));
-          *reinterpret_cast<uint4*>(p_ptr + h * 128 + ((c ^ (h & 7)) << 4)) = v;
-        }
+      for (int j = 0; j < 8; ++j) {
+        const float got = __shfl_xor_sync(0xffffffffu, odd ? s[j] : s[j + 8], 2);
+        w[j] = odd ? pack2<T>(got, s[j + 8]) : pack2<T>(s[j], got);
       }
+      // their buffer is free once the product of the tile before the last has read it
+      if (it > 1) wait(&sh.pv_done[it & 1], (it - 2) >> 1);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<uint4*>(p_ptr + h * 128 + ((((it & 1) * 4 + odd * 2 + c) ^ (h & 7)) << 4)) =
+            make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
       fence_async_shared();
       tc_fence_before();
-      mbar_arrive(&sh.p_full);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[it & 3]);
 
       if (at.last() || it == n - 1) {
-        wait(&sh.pv_done, it);
+        wait(&sh.pv_done[it & 1], it >> 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
         tc_fence_after();
         const bool whole = at.last() && segment_tile == 0;   // all of the row's tiles were here
         const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (segment > 0 ? 1 : 0));
@@ -403,28 +431,31 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     }
   } else if (warp < 12) {
     // ---------------- producers ----------------
-    const int set = (warp - 4) >> 2, w = warp & 3;
-    int s = set, turn = 0;                       // the number of stages is even
+    const int set = (warp - 4) >> 1, w = warp & 1;
+    int s = set, turn = 0;                       // the number of stages is a multiple of the sets'
     for (int i = 0; i < set && i < n; ++i) at.next(a);
     int64_t slot = set < n && lane < 16 ? slot_of(a, at.row, at.tile * static_cast<int64_t>(kTile) + 16 * w + lane) : -1;
-    for (int it = set; it < n; it += 2) {
+    for (int it = set; it < n; it += kSets) {
       if (!mbar_wait(&sh.empty[s], (turn & 1) ^ 1, &sh.abort, kWaitNs)) {
         give_up(sh, a.status);
         break;
       }
       const unsigned some = __ballot_sync(0xffffffffu, slot >= 0) & 0xFFFFu;
       if (lane == 0) reinterpret_cast<volatile uint16_t*>(&sh.mask[s])[w] = static_cast<uint16_t>(some);
+      if (lane == 0 && w == 0)
+        *reinterpret_cast<volatile uint32_t*>(&sh.flags[s]) = (it == 0 || at.first() ? 1 : 0) | (at.last() ? 2 : 0);
       const char* src = slot >= 0 ? static_cast<const char*>(a.pool) + slot * a.pool_stride * 2 : nullptr;
-      copy_rows<kChunks>(kv_smem + s * kChunks * kBlock, src, a.q, 16 * w, lane);
-      if (it + 2 < n) {   // the next tile's slots arrive while this one's rows do
-        at.next(a);
-        at.next(a);
+      copy_rows<kChunks, kBlock>(kv_smem + s * kChunks * kBlock, src, a.q, 16 * w, lane);
+      if (it + kSets < n) {   // the next tile's slots arrive while this one's rows do
+#pragma unroll
+        for (int i = 0; i < kSets; ++i) at.next(a);
         slot = lane < 16 ? slot_of(a, at.row, at.tile * static_cast<int64_t>(kTile) + 16 * w + lane) : -1;
       }
       cp_async_wait_all();
       fence_async_shared();
-      mbar_arrive(&sh.full[s]);
-      s += 2;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.full[s]);
+      s += kSets;
       if (s >= a.stages) {
         s = set;
         ++turn;
@@ -432,74 +463,50 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     }
     cp_async_wait_all();
   } else if (warp == 12) {
-    // ---------------- MMA issuer ----------------
-    if (n > 0) {
-      const uint32_t qk = idesc_16bit_f32(kBf16, 64, 64, false, false);
-      const uint32_t pv = idesc_16bit_f32(kBf16, 128, (heads + 15) & ~15, true, false);
-      const uint32_t q_desc = desc_k(q_smem), p_desc = desc_k(p_smem);
-      Place ahead = at;                          // the tile whose scores are issued next
-      int scored = 0, done = 0, rows_scored = 0;
-      int s_stage = 0, s_turn = 0, o_stage = 0;
-      uint64_t t_idle = 0;
-      uint32_t spins = 0;
-      while (done < n) {
-        bool moved = false;
-        if (scored < n && scored <= done + 1) {
-          const bool fresh = scored == 0 || ahead.first();
-          if (__all_sync(0xffffffffu, mbar_test(&sh.full[s_stage], s_turn & 1) &&
-                                          (!fresh || mbar_test(&sh.q_full, rows_scored & 1)))) {
-            tc_fence_after();
-            const uint32_t k_desc = desc_k(kv_smem + s_stage * kChunks * kBlock), d = tmem + kScoreCol + (scored & 1) * 64;
+    // ---------------- scores ----------------
+    const uint32_t qk = idesc_16bit_f32(kBf16, kGroup, kTile, false, false), q_desc = desc_k(q_smem);
+    int rows_scored = 0, s = 0, turn = 0, scored = 0;
+    for (int it = 0; it < n; ++it, ++scored) {
+      if (it >= 4 && !converged_wait(sh, a.status, &sh.p_full[it & 3], (it - 4) >> 2)) break;   // S is free again
+      if (!converged_wait(sh, a.status, &sh.full[s], turn)) break;
+      const uint32_t flags = *reinterpret_cast<volatile uint32_t*>(&sh.flags[s]);
+      if (__any_sync(0xffffffffu, flags & 1) && !converged_wait(sh, a.status, &sh.q_full, rows_scored++)) break;
+      const uint32_t k_desc = desc_k(kv_smem + s * kChunks * kBlock), d = tmem + kScoreCol + (it & 3) * kTile;
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c)
+      for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16(d, q_desc + (c * kBlock + 32 * k) / 16, k_desc + (c * kBlock + 32 * k) / 16, qk, c + k > 0 ? 1u : 0u);
-            umma_commit_elect(&sh.s_full[scored & 1]);
-            if (fresh) ++rows_scored;
-            if (ahead.last()) umma_commit_elect(&sh.q_empty);
-            ahead.next(a);
-            if (++s_stage == a.stages) {
-              s_stage = 0;
-              ++s_turn;
-            }
-            ++scored;
-            moved = true;
-          }
-        }
-        if (done < scored && __all_sync(0xffffffffu, mbar_test(&sh.p_full, done & 1))) {
-          tc_fence_after();
-          const uint32_t v_desc = desc_mn(kv_smem + o_stage * kChunks * kBlock, kBlock);
-          const uint32_t more = done == 0 || at.first() ? 0u : 1u;
-#pragma unroll
-          for (int t = 0; t < kOut; ++t)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16(tmem + t * 64, v_desc + (2 * t * kBlock + 2048 * k) / 16, p_desc + 32 * k / 16, pv, k > 0 ? 1u : more);
-          umma_commit_elect(&sh.empty[o_stage]);
-          umma_commit_elect(&sh.pv_done);
-          at.next(a);
-          if (++o_stage == a.stages) o_stage = 0;
-          ++done;
-          moved = true;
-        }
-        if (moved) {
-          t_idle = 0;
-        } else if ((++spins & 63) == 0) {
-          const uint64_t t = globaltimer_ns();
-          if (!t_idle) t_idle = t;
-          const bool late = t - t_idle > kWaitNs;
-          if (late) give_up(sh, a.status);
-          if (__any_sync(0xffffffffu, late || *reinterpret_cast<volatile int*>(&sh.abort))) break;
-        }
+        for (int k = 0; k < 4; ++k)
+          umma_f16(d, q_desc + (c * kQBlock + 32 * k) / 16, k_desc + (c * kBlock + 32 * k) / 16, qk, c + k > 0 ? 1u : 0u);
+      umma_commit_elect(&sh.s_full[it & 3]);
+      if (__any_sync(0xffffffffu, flags & 2)) umma_commit_elect(&sh.q_empty);
+      if (++s == a.stages) {
+        s = 0;
+        ++turn;
       }
-      // everything that was issued retires before the CTA ends
-      if (scored > 0) mbar_wait(&sh.s_full[(scored - 1) & 1], ((scored - 1) >> 1) & 1, &sh.zero, kWaitNs);
-      if (done > 0) {
-        const int last = done - 1;
-        mbar_wait(&sh.empty[last % a.stages], (last / a.stages) & 1, &sh.zero, kWaitNs);
-        mbar_wait(&sh.pv_done, (done - 1) & 1, &sh.zero, kWaitNs);
-      }
+    }
+    // what was issued retires before the CTA ends
+    if (scored > 0) mbar_wait(&sh.s_full[(scored - 1) & 3], ((scored - 1) >> 2) & 1, &sh.zero, kWaitNs);
+  } else if (warp == 13) {
+    // ---------------- output ----------------
+    const uint32_t pv = idesc_16bit_f32(kBf16, 128, (heads + 15) & ~15, true, false), p_desc = desc_k(p_smem);
+    int s = 0, done = 0;
+    for (int it = 0; it < n; ++it, ++done) {
+      if (!converged_wait(sh, a.status, &sh.p_full[it & 3], it >> 2)) break;
+      const uint32_t more = (*reinterpret_cast<volatile uint32_t*>(&sh.flags[s]) & 1) ^ 1;
+      const uint32_t v_desc = desc_mn(kv_smem + s * kChunks * kBlock, kBlock), p = p_desc + (it & 1) * 64 / 16;
+#pragma unroll
+      for (int t = 0; t < kOut; ++t)
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_f16(tmem + t * 64, v_desc + (2 * t * kBlock + 2048 * k) / 16, p + 32 * k / 16, pv, k > 0 ? 1u : more);
+      umma_commit_elect(&sh.empty[s]);
+      umma_commit_elect(&sh.pv_done[it & 1]);
+      if (++s == a.stages) s = 0;
+    }
+    if (done > 0) {
+      const int last = done - 1;
+      mbar_wait(&sh.empty[last % a.stages], (last / a.stages) & 1, &sh.zero, kWaitNs);
+      mbar_wait(&sh.pv_done[last & 1], (last >> 1) & 1, &sh.zero, kWaitNs);
     }
   } else {
     // ---------------- queries ----------------
@@ -512,11 +519,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       const char* q = static_cast<const char*>(a.q) + (at.row * a.qs0 + group * kGroup * a.qs1) * 2;
       for (int w = 0; w < 4; ++w) {
         const int hh = 16 * w + lane;
-        copy_rows<kChunks>(q_smem, lane < 16 && hh < heads ? q + hh * a.qs1 * 2 : nullptr, a.q, 16 * w, lane);
+        copy_rows<kChunks, kQBlock>(q_smem, lane < 16 && hh < heads ? q + hh * a.qs1 * 2 : nullptr, a.q, 16 * w, lane);
       }
       cp_async_wait_all();
       fence_async_shared();
-      mbar_arrive(&sh.q_full);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full);
       ++rows_loaded;
       it += at.tiles - at.tile;
       at.tile = at.tiles - 1;
@@ -610,12 +618,12 @@ int64_t ranges_for(int64_t rows, int64_t heads, int64_t count) {
 // Launches the kernels of one element type and one pair of widths.
 template <typename T, int kLatent, int kRope>
 void launch(LatentArgs a, cudaStream_t s) {
-  constexpr int64_t kFixed = kBlock + 1024 + static_cast<int64_t>(sizeof(LatentShared));
-  constexpr int64_t kStage = (kLatent + kRope) / 64 * kBlock;
-  constexpr int64_t kFit = (kMaxSmem - kFixed) / kStage - 1;
-  constexpr int kStages = static_cast<int>(kFit > kMaxStages ? kMaxStages : kFit & ~int64_t(1));
-  static_assert(kStages >= 2, "two stages at least");
-  constexpr int64_t kSmem = kFixed + (1 + kStages) * kStage;
+  constexpr int kChunks = (kLatent + kRope) / 64;
+  constexpr int64_t kFixed = kChunks * kQBlock + kPBytes + 1024 + static_cast<int64_t>(sizeof(LatentShared));
+  constexpr int kStages = kFixed + 2 * kSets * kChunks * kBlock <= kMaxSmem ? 2 * kSets : kSets;
+  static_assert(kStages <= kMaxStages, "barriers");
+  constexpr int64_t kSmem = kFixed + static_cast<int64_t>(kStages) * kChunks * kBlock;
+  static_assert(kSmem <= kMaxSmem, "shared memory");
   a.stages = kStages;
   static DeviceOnce once;
   once.run([] {
