@@ -70,7 +70,7 @@ SIGNATURES = {
     "v1x_route_pages": [P, I64, P, P, P, I32, I64, I64, P, P, I64, P, I64, I32, I64, P],
     "v1x_gather_slots": [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64,
                          P],
-    "v1x_latent_attention_workspace": [I64, I64, I64, I64],
+    "v1x_latent_attention_workspace": [I64, I64, I64, I64, I32],
     "v1x_latent_attention": [P, I64, I64, P, I64, I64, P, I64, P, I64, I64, P, I64, I64, I64, I64, F32, I32, P, P, P,
                              I64, P, P],
     "v1x_prompt_attention": [P, I64, I64, P, I64, I64, P, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, F32, I32, P,

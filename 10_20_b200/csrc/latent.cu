@@ -2,42 +2,42 @@
 // in v1x.h.
 //
 // Every head reads the same rows, as keys (all of a row) and as values (its first
-// `latent` elements), so a tile of 32 tokens is brought into shared memory once
+// `latent` elements), so a tile of 64 tokens is brought into shared memory once
 // and is an operand of both products:
 //
-//   S[64 heads x 32 tokens]      = Q . K^T        M = 64, N = 32, K = dim
-//   O^T[128 of latent x heads]  += V^T . P^T      M = 128, N = heads, K = 32
+//   S[64 heads x 64 tokens]      = Q . K^T        M = 64, N = 64, K = dim
+//   O^T[128 of latent x heads]  += V^T . P^T      M = 128, N = heads, K = 64
 //
 // The output is kept transposed because its M is then the latent width, full
 // 128-row operands for any number of heads, and its four accumulators of 64
-// columns leave room for the score tiles.  The same bytes serve as K-major (keys)
+// columns leave room for two score tiles.  The same bytes serve as K-major (keys)
 // and MN-major (values) operand.  Softmax in one pass, in powers of two: the
 // running maximum that the weights are taken against moves only when a tile
 // exceeds it by more than 2^8, so that O is rescaled a few times a row at most;
 // sums stay in 32 bits, the weights are rounded once, to the inputs' type, for the
 // second product.
 //
-// What bounds it: 72 KB of queries leave room for 144 KB of tokens, and a stage is
-// held from its first load to its last product, a chain of latencies (load,
-// scores, softmax, product).  Four stages of 32 tokens turn around faster than two
-// of 64 (DECODE64 -> DECODE32 us on the decode batch), although N = 32 costs the
-// scores' product a quarter of its rate.
+// What bounds it: 72 KB of queries leave room for 144 KB of tokens, two tiles, and
+// a tile is held from its first load to its last product, a chain of latencies
+// (load, scores, softmax, output).  So a tile is loaded and released in two halves
+// of 32 tokens.
 //
 // Work: the tiles of all rows in a line, cut into equal ranges, one CTA each (times
 // the groups of 64 heads, neighbours in the grid, which read the same tiles at the
 // same time from L2).  A row that lies in several ranges leaves unnormalised parts
-// in the workspace, joined by latent_join_kernel in the order of the ranges.
+// in the workspace, joined by latent_join_kernel in the order of the ranges; rows
+// of equal length are given to the CTAs whole where that is no longer (cut_for).
 //
 // Warp roles (480 threads, one CTA per SM):
 //   0-3   softmax, rescale, epilogue (TMEM lane quarters 0-3)
-//   4-11  four sets of two producer warps, every fourth tile: rows by 16-byte
-//         cp.async into the swizzled layout, each row's slot looked up a tile
-//         ahead; a token that is none becomes zeros and a cleared bit of the
+//   4-11  four sets of two producer warps, a half of every other tile each: rows by
+//         16-byte cp.async into the swizzled layout, each row's slot looked up a
+//         tile ahead; a token that is none becomes zeros and a cleared bit of the
 //         tile's mask
-//   12    TMEM owner; issues the scores' MMAs, up to four tiles ahead
-//   13    issues the outputs' MMAs: an MMA of these shapes takes 24 to 48 cycles and few
-//         are queued, so that one warp's waits between the products would leave the
-//         tensor cores idle (ONEWARP -> TWOWARPS us on the decode batch)
+//   12    TMEM owner; issues the scores' MMAs, up to two tiles ahead
+//   13    issues the outputs' MMAs: an MMA of these shapes takes 32 to 48 cycles and
+//         few are queued, so one warp's waits between the two products left the
+//         tensor cores idle (111 us instead of 92 on the decode batch)
 //   14    the queries, when the row changes
 // Waits are bounded (2 s, then V1X_STATUS_TIMEOUT).
 #include <type_traits>
@@ -51,13 +51,10 @@ namespace {
 using namespace attn;
 using namespace sm100;
 
-constexpr int kTile = 32;                // tokens of a tile
+constexpr int kTile = 64;                // tokens of a tile, in two halves
 constexpr int kGroup = 64;               // heads of a CTA
-constexpr int kQBlock = kGroup * 128;    // bytes of 64 elements of a tile's rows: queries, ...
-constexpr int kBlock = kTile * 128;      // ... tokens
-constexpr int kPBytes = kGroup * 128;    // two tiles' weights side by side in 128-byte rows
-constexpr int kSets = 4;                 // producer sets, two warps each
-constexpr int kMaxStages = 8;
+constexpr int kBlock = 64 * 128;         // bytes of 64 elements of 64 rows (queries, tokens) or of the weights
+constexpr int kMaxPairs = 4;             // tiles in shared memory: 2, or 4 where they fit
 constexpr int kThreads = 480;
 constexpr int kMaxCtas = 148;
 constexpr uint32_t kScoreCol = 256;      // TMEM: O^T in columns 0-255, two score tiles after it
@@ -75,7 +72,8 @@ struct LatentArgs {
   int64_t index_stride, count;
   const int32_t* lens;
   int64_t rows, heads;
-  int stages, groups, ranges;
+  int pairs, groups, ranges;
+  int64_t unit, base, extra;   // the cut of the line in units of `unit` tiles (lens: unit 1, on the device)
   float scale_log2;
   void* out;
   float* lse;
@@ -87,10 +85,14 @@ struct LatentArgs {
 };
 
 struct LatentShared {
-  uint64_t full[kMaxStages], empty[kMaxStages], s_full[4], p_full[4], pv_done[2], q_full, q_empty;
-  uint32_t mask[kMaxStages], flags[kMaxStages];   // flags: 1 the first tile of a segment, 2 the last of a row
+  uint64_t full[2 * kMaxPairs];    // of a tile: its first blocks, all of it
+  uint64_t empty[2 * kMaxPairs];   // its halves
+  uint64_t s_full[2], p_full[2], pv_done, q_full, q_empty;
+  uint64_t mask[kMaxPairs];
+  uint32_t flags[kMaxPairs];   // 1: the first tile of a segment, 2: the last of a row
   float factor[kGroup];
-  int64_t start[4];  // as LatentArgs::where
+  int64_t start[4];  // as LatentArgs::where, but [3]: all tiles
+  int64_t cut[2];    // base, extra
   int64_t scan[kThreads / 32 + 1];
   uint32_t tmem;
   int abort, zero;
@@ -130,7 +132,10 @@ __device__ __forceinline__ int64_t slot_of(const LatentArgs& a, int64_t r, int64
   return s >= 0 && s < a.slots ? s : -1;
 }
 
-__device__ __forceinline__ int64_t range_start(int64_t tiles, int64_t x, int64_t ranges) { return tiles * x / ranges; }
+// The first tile of range x: ranges of `base` units, the first `extra` of them one more.
+__device__ __forceinline__ int64_t range_start(int64_t x, int64_t unit, int64_t base, int64_t extra) {
+  return (x * base + min(x, extra)) * unit;
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -163,42 +168,46 @@ __device__ __forceinline__ bool any_of_128(bool x) {
 }
 __device__ __forceinline__ void sync_128() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
-// Rows of kChunks 64-element blocks into the swizzled operand layout: row R of
-// block c at c * kBytes + R * 128, its 16-byte pieces permuted by R & 7.
-// A group of eight lanes moves one 128-byte piece of a row at a time; the warp
-// covers the 16 rows R0 .. R0 + 15, whose sources `src` (per lane l < 16: row R0 + l,
-// null for zeros, `any` then being an address that is not read) are handed over by
-// shuffles.
-template <int kChunks, int kBytes>
-__device__ __forceinline__ void copy_rows(uint32_t dst, const char* src, const void* any, int R0, int lane) {
+// Rows into the swizzled operand layout, 64 elements a block: row R of block c at
+// c * kBlock + R * 128, its 16-byte pieces permuted by R & 7.  A group of eight
+// lanes moves one 128-byte piece of a row at a time; the warp covers the 16 rows
+// R0 .. R0 + 15, whose sources (per lane l < 16: row R0 + l, null for zeros, `any`
+// then being an address that is not read) are handed over by shuffles.
+struct RowCopy {
   const char* from[4];
   uint32_t to[4], bytes[4];
+  __device__ __forceinline__ RowCopy(uint32_t dst, const char* src, const void* any, int R0, int lane) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = 4 * i + (lane >> 3), R = R0 + row;
-    const char* p = reinterpret_cast<const char*>(
-        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), row));
-    bytes[i] = p ? 16 : 0;
-    from[i] = p ? p + (lane & 7) * 16 : static_cast<const char*>(any);
-    to[i] = dst + R * 128 + (((lane & 7) ^ (R & 7)) << 4);
+    for (int i = 0; i < 4; ++i) {
+      const int row = 4 * i + (lane >> 3), R = R0 + row;
+      const char* p = reinterpret_cast<const char*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), row));
+      bytes[i] = p ? 16 : 0;
+      from[i] = p ? p + (lane & 7) * 16 : static_cast<const char*>(any);
+      to[i] = dst + R * 128 + (((lane & 7) ^ (R & 7)) << 4);
+    }
   }
+  template <int kBegin, int kEnd>
+  __device__ __forceinline__ void blocks() const {
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c)
+    for (int c = kBegin; c < kEnd; ++c)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) cp_async16(to[i] + c * kBytes, from[i] + c * 128, bytes[i]);
-}
+      for (int i = 0; i < 4; ++i) cp_async16(to[i] + c * kBlock, from[i] + c * 128, bytes[i]);
+  }
+};
 
 template <typename T, int kLatent, int kRope>
 __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_constant__ LatentArgs a) {
   constexpr int kChunks = (kLatent + kRope) / 64, kOut = kLatent / 128;
+  constexpr int kEarly = (kChunks + 1) / 2;   // the blocks that the scores begin with
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t q_smem = smem_u32(base);
-  const uint32_t kv_smem = q_smem + kChunks * kQBlock;
-  uint8_t* p_ptr = base + kChunks * (kQBlock + a.stages * kBlock);
+  const uint32_t kv_smem = q_smem + kChunks * kBlock;
+  uint8_t* p_ptr = base + kChunks * (1 + a.pairs) * kBlock;
   const uint32_t p_smem = smem_u32(p_ptr);
-  LatentShared& sh = *reinterpret_cast<LatentShared*>(p_ptr + kPBytes);
+  LatentShared& sh = *reinterpret_cast<LatentShared*>(p_ptr + kBlock);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = blockIdx.x % a.groups;
   const int64_t x = blockIdx.x / a.groups;
@@ -207,15 +216,15 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   if (tid == 0) {
     sh.abort = 0;
     sh.zero = 0;
-    for (int s = 0; s < a.stages; ++s) {
-      mbar_init(&sh.full[s], 2);
+    for (int s = 0; s < 2 * a.pairs; ++s) {
+      mbar_init(&sh.full[s], 4);
       mbar_init(&sh.empty[s], 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 4);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&sh.pv_done[i], 1);
+    mbar_init(&sh.pv_done, 1);
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1);
     fence_mbar_init();
@@ -226,23 +235,33 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     tc_fence_before();
   }
   // ---- this CTA's range of the line ---------------------------------------------
-  if (tid == 0) {
-    const int64_t per = a.lens ? 0 : (a.count + kTile - 1) / kTile, all = per * a.rows;
-    const int64_t row = per ? range_start(all, x, a.ranges) / per : 0;
-    sh.start[0] = row;
-    sh.start[1] = row * per;
-    sh.start[2] = per ? per : 1;
-    sh.start[3] = all;
-  }
-  __syncthreads();
-  if (a.lens) {
+  if (!a.lens) {
+    if (tid == 0) {
+      const int64_t per = (a.count + kTile - 1) / kTile, t0 = range_start(x, a.unit, a.base, a.extra);
+      const int64_t row = per ? (t0 >> 31 ? t0 / per : static_cast<uint32_t>(t0) / static_cast<uint32_t>(per)) : 0;
+      sh.start[0] = row;
+      sh.start[1] = row * per;
+      sh.start[2] = per;
+      sh.start[3] = per * a.rows;
+      sh.cut[0] = a.base;
+      sh.cut[1] = a.extra;
+    }
+    __syncthreads();
+  } else {
     const int64_t chunk = (a.rows + kThreads - 1) / kThreads;
     const int64_t beg = min(tid * chunk, a.rows), end = min(beg + chunk, a.rows);
     int64_t mine = 0, all;
     for (int64_t r = beg; r < end; ++r) mine += row_tiles(a, r);
     int64_t run = block_exclusive_scan(mine, sh.scan, &all);
-    const int64_t t0 = range_start(all, x, a.ranges);
-    if (tid == 0) sh.start[3] = all;
+    if (tid == 0) {
+      sh.start[0] = sh.start[1] = 0;
+      sh.start[2] = 1;
+      sh.start[3] = all;
+      sh.cut[0] = all >> 31 ? all / a.ranges : static_cast<uint32_t>(all) / static_cast<uint32_t>(a.ranges);
+      sh.cut[1] = all - sh.cut[0] * a.ranges;
+    }
+    __syncthreads();
+    const int64_t t0 = range_start(x, 1, sh.cut[0], sh.cut[1]);
     if (run <= t0 && t0 < run + mine) {
       for (int64_t r = beg; r < end; ++r) {
         const int64_t n = row_tiles(a, r);
@@ -259,8 +278,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   }
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  const int64_t t0 = range_start(sh.start[3], x, a.ranges);
-  const int n = static_cast<int>(range_start(sh.start[3], x + 1, a.ranges) - t0);   // tiles of the range
+  const int64_t t0 = range_start(x, a.unit, sh.cut[0], sh.cut[1]);
+  const int n = static_cast<int>(range_start(x + 1, a.unit, sh.cut[0], sh.cut[1]) - t0);   // tiles of the range
   Place at{static_cast<int>(sh.start[0]), static_cast<int>(t0 - sh.start[1]), static_cast<int>(sh.start[2])};
   if (tid == 0 && group == 0 && a.where) {
     for (int i = 0; i < 3; ++i) a.where[4 * x + i] = sh.start[i];
@@ -278,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     const int cols = (heads + 31) & ~31;         // accumulator columns moved, 32 at a time
     float m = -CUDART_INF_F, l = 0.0f;
     bool fresh = true;                           // the tile begins a segment: tiles of one row in this range
-    int segment = 0, segment_tile = 0, stage = 0, turn = 0;
+    int segment = 0, segment_tile = 0, pair = 0, turn = 0;
     // after a wait that gave up the loop goes on without waiting, so that all
     // four warps still meet at their barriers
     bool ok = true;
@@ -289,28 +308,29 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       }
     };
     for (int it = 0; it < n; ++it) {
-      wait(&sh.s_full[it & 3], it >> 2);
-      wait(&sh.full[stage], turn);               // complete already: the producers' mask
+      wait(&sh.s_full[it & 1], it >> 1);
       tc_fence_after();
-      uint32_t raw[16];
-      tmem_ld16x32(tmem + quarter + kScoreCol + (it & 3) * kTile, raw);
-      const uint32_t valid = *reinterpret_cast<volatile uint32_t*>(&sh.mask[stage]);
-      if (++stage == a.stages) {
-        stage = 0;
+      uint32_t raw[32];
+      tmem_ld16x64(tmem + quarter + kScoreCol + (it & 1) * kTile, raw);
+      wait(&sh.full[2 * pair], turn);            // complete already: the producers' mask
+      const uint64_t valid = *reinterpret_cast<volatile uint64_t*>(&sh.mask[pair]);
+      if (++pair == a.pairs) {
+        pair = 0;
         ++turn;
       }
       tmem_ld_wait();
-      float s[16];
+      float s[32];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = __uint_as_float(raw[j]) * a.scale_log2;
-      if (valid != ~0u) {
+      for (int j = 0; j < 32; ++j) s[j] = __uint_as_float(raw[j]) * a.scale_log2;
+      if (valid != ~0ull) {
+        const uint64_t own = valid >> odd;
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (!((valid >> (2 * j + odd)) & 1)) s[j] = -CUDART_INF_F;
+        for (int j = 0; j < 32; ++j)
+          if (!((own >> (2 * j)) & 1)) s[j] = -CUDART_INF_F;
       }
       float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int j = 4; j < 16; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
+      for (int j = 4; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
       float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       if (fresh) {
@@ -324,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
           if (grows) m = most;
           l *= f;
           if (mine) sh.factor[h] = f;
-          wait(&sh.pv_done[(it - 1) & 1], (it - 1) >> 1);
+          wait(&sh.pv_done, it - 1);
           sync_128();
           tc_fence_after();
           for (int t = 0; t < kOut; ++t)
@@ -344,32 +364,32 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       const float ref = m == -CUDART_INF_F ? 0.0f : m;
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < 32; ++j) {
         s[j] = exp2_fast(s[j] - ref);
         sum[j & 3] += s[j];
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      // neighbouring tokens' weights meet in one thread: tokens 0-15 of the tile in
-      // the even one, 16-31 in the odd one
-      uint32_t w[8];
+      // neighbouring tokens' weights meet in one thread: tokens 0-31 of the tile in
+      // the even one, 32-63 in the odd one
+      uint32_t w[16];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float got = __shfl_xor_sync(0xffffffffu, odd ? s[j] : s[j + 8], 2);
-        w[j] = odd ? pack2<T>(got, s[j + 8]) : pack2<T>(s[j], got);
+      for (int j = 0; j < 16; ++j) {
+        const float got = __shfl_xor_sync(0xffffffffu, odd ? s[j] : s[j + 16], 2);
+        w[j] = odd ? pack2<T>(got, s[j + 16]) : pack2<T>(s[j], got);
       }
-      // their buffer is free once the product of the tile before the last has read it
-      if (it > 1) wait(&sh.pv_done[it & 1], (it - 2) >> 1);
+      // their buffer is free once the previous tile's product has read it
+      if (it > 0) wait(&sh.pv_done, it - 1);
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<uint4*>(p_ptr + h * 128 + ((((it & 1) * 4 + odd * 2 + c) ^ (h & 7)) << 4)) =
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(p_ptr + h * 128 + (((odd * 4 + c) ^ (h & 7)) << 4)) =
             make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
       fence_async_shared();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full[it & 3]);
+      if (lane == 0) mbar_arrive(&sh.p_full[it & 1]);
 
       if (at.last() || it == n - 1) {
-        wait(&sh.pv_done[it & 1], it >> 1);
+        wait(&sh.pv_done, it);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         tc_fence_after();
         const bool whole = at.last() && segment_tile == 0;   // all of the row's tiles were here
@@ -396,16 +416,25 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
             tmem_ld_wait();
             const int d = t * 128 + warp * 32 + lane, left = heads - c;
             if (whole) {
-              // lane pairs exchange, so that a lane has two neighbours of one head
-              T* const to = out + c * kLatent + (lane & 1) * kLatent + (d & ~1);
+              // 32 heads x 128 columns through the weights' buffer (free: the last product
+              // has read it), so that a head's 256 bytes are written as one piece
+              uint16_t* const stage = reinterpret_cast<uint16_t*>(p_ptr) + warp * 32 + lane;
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
-                const float u = __uint_as_float(o[j]) * sh.factor[c + j];
-                const float v = __uint_as_float(o[j + 1]) * sh.factor[c + j + 1];
-                const float y = __shfl_xor_sync(0xffffffffu, lane & 1 ? u : v, 1);
-                const uint32_t two = lane & 1 ? pack2<T>(y, v) : pack2<T>(u, y);
-                if (j + (lane & 1) < left) *reinterpret_cast<uint32_t*>(to + j * kLatent) = two;
+                const uint32_t two = pack2<T>(__uint_as_float(o[j]) * sh.factor[c + j],
+                                              __uint_as_float(o[j + 1]) * sh.factor[c + j + 1]);
+                stage[j * 128] = static_cast<uint16_t>(two);
+                stage[(j + 1) * 128] = static_cast<uint16_t>(two >> 16);
               }
+              sync_128();
+              T* const to = out + static_cast<int64_t>(c) * kLatent + t * 128;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int hh = 8 * i + (tid >> 4), e = (tid & 15) * 8;
+                if (hh < left)
+                  *reinterpret_cast<uint4*>(to + hh * kLatent + e) = *reinterpret_cast<const uint4*>(p_ptr + hh * 256 + e * 2);
+              }
+              sync_128();
             } else {
               float* const to = part + c * kLatent + d;
 #pragma unroll
@@ -431,33 +460,47 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     }
   } else if (warp < 12) {
     // ---------------- producers ----------------
-    const int set = (warp - 4) >> 1, w = warp & 1;
-    int s = set, turn = 0;                       // the number of stages is a multiple of the sets'
-    for (int i = 0; i < set && i < n; ++i) at.next(a);
-    int64_t slot = set < n && lane < 16 ? slot_of(a, at.row, at.tile * static_cast<int64_t>(kTile) + 16 * w + lane) : -1;
-    for (int it = set; it < n; it += kSets) {
-      if (!mbar_wait(&sh.empty[s], (turn & 1) ^ 1, &sh.abort, kWaitNs)) {
+    const int half = (warp >> 1) & 1, turn_of = (warp - 4) >> 2, R0 = 32 * half + 16 * (warp & 1);
+    int pair = turn_of, turn = 0;                // tiles turn_of, turn_of + 2, ...; the number of pairs is even
+    if (turn_of < n)
+      for (int i = 0; i < turn_of; ++i) at.next(a);
+    auto slot_ahead = [&] {
+      return lane < 16 ? slot_of(a, at.row, at.tile * static_cast<int64_t>(kTile) + R0 + lane) : -1;
+    };
+    int64_t slot = turn_of < n ? slot_ahead() : -1;
+    for (int it = turn_of; it < n; it += 2) {
+      if (!mbar_wait(&sh.empty[2 * pair + half], (turn & 1) ^ 1, &sh.abort, kWaitNs)) {
         give_up(sh, a.status);
         break;
       }
       const unsigned some = __ballot_sync(0xffffffffu, slot >= 0) & 0xFFFFu;
-      if (lane == 0) reinterpret_cast<volatile uint16_t*>(&sh.mask[s])[w] = static_cast<uint16_t>(some);
-      if (lane == 0 && w == 0)
-        *reinterpret_cast<volatile uint32_t*>(&sh.flags[s]) = (it == 0 || at.first() ? 1 : 0) | (at.last() ? 2 : 0);
-      const char* src = slot >= 0 ? static_cast<const char*>(a.pool) + slot * a.pool_stride * 2 : nullptr;
-      copy_rows<kChunks, kBlock>(kv_smem + s * kChunks * kBlock, src, a.q, 16 * w, lane);
-      if (it + kSets < n) {   // the next tile's slots arrive while this one's rows do
-#pragma unroll
-        for (int i = 0; i < kSets; ++i) at.next(a);
-        slot = lane < 16 ? slot_of(a, at.row, at.tile * static_cast<int64_t>(kTile) + 16 * w + lane) : -1;
+      if (lane == 0) {
+        reinterpret_cast<volatile uint16_t*>(&sh.mask[pair])[R0 >> 4] = static_cast<uint16_t>(some);
+        if (R0 == 0)
+          *reinterpret_cast<volatile uint32_t*>(&sh.flags[pair]) = (it == 0 || at.first() ? 1 : 0) | (at.last() ? 2 : 0);
       }
-      cp_async_wait_all();
+      const char* src = slot >= 0 ? static_cast<const char*>(a.pool) + slot * a.pool_stride * 2 : nullptr;
+      const RowCopy copy(kv_smem + pair * kChunks * kBlock, src, a.q, R0, lane);
+      copy.template blocks<0, kEarly>();
+      cp_async_commit();
+      copy.template blocks<kEarly, kChunks>();
+      cp_async_commit();
+      if (it + 2 < n) {   // the next tile's slots arrive while this one's rows do
+        at.next(a);
+        at.next(a);
+        slot = slot_ahead();
+      }
+      cp_async_wait<1>();
       fence_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.full[s]);
-      s += kSets;
-      if (s >= a.stages) {
-        s = set;
+      if (lane == 0) mbar_arrive(&sh.full[2 * pair]);
+      cp_async_wait<0>();
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.full[2 * pair + 1]);
+      pair += 2;
+      if (pair >= a.pairs) {
+        pair = turn_of;
         ++turn;
       }
     }
@@ -465,48 +508,65 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   } else if (warp == 12) {
     // ---------------- scores ----------------
     const uint32_t qk = idesc_16bit_f32(kBf16, kGroup, kTile, false, false), q_desc = desc_k(q_smem);
-    int rows_scored = 0, s = 0, turn = 0, scored = 0;
+    int rows_scored = 0, pair = 0, turn = 0, scored = 0;
     for (int it = 0; it < n; ++it, ++scored) {
-      if (it >= 4 && !converged_wait(sh, a.status, &sh.p_full[it & 3], (it - 4) >> 2)) break;   // S is free again
-      if (!converged_wait(sh, a.status, &sh.full[s], turn)) break;
-      const uint32_t flags = *reinterpret_cast<volatile uint32_t*>(&sh.flags[s]);
+      if (it >= 2 && !converged_wait(sh, a.status, &sh.p_full[it & 1], (it - 2) >> 1)) break;   // S is free again
+      if (!converged_wait(sh, a.status, &sh.full[2 * pair], turn)) break;
+      const uint32_t flags = *reinterpret_cast<volatile uint32_t*>(&sh.flags[pair]);
       if (__any_sync(0xffffffffu, flags & 1) && !converged_wait(sh, a.status, &sh.q_full, rows_scored++)) break;
-      const uint32_t k_desc = desc_k(kv_smem + s * kChunks * kBlock), d = tmem + kScoreCol + (it & 3) * kTile;
+      const uint32_t k_desc = desc_k(kv_smem + pair * kChunks * kBlock), d = tmem + kScoreCol + (it & 1) * kTile;
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)
+      for (int c = 0; c < kEarly; ++c)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_f16(d, q_desc + (c * kQBlock + 32 * k) / 16, k_desc + (c * kBlock + 32 * k) / 16, qk, c + k > 0 ? 1u : 0u);
-      umma_commit_elect(&sh.s_full[it & 3]);
+          umma_f16(d, q_desc + (c * kBlock + 32 * k) / 16, k_desc + (c * kBlock + 32 * k) / 16, qk, c + k > 0 ? 1u : 0u);
+      if (!converged_wait(sh, a.status, &sh.full[2 * pair + 1], turn)) {
+        umma_commit_elect(&sh.s_full[it & 1]);   // what was issued is waited for below
+        ++scored;
+        break;
+      }
+#pragma unroll
+      for (int c = kEarly; c < kChunks; ++c)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_f16(d, q_desc + (c * kBlock + 32 * k) / 16, k_desc + (c * kBlock + 32 * k) / 16, qk, c + k > 0 ? 1u : 0u);
+      umma_commit_elect(&sh.s_full[it & 1]);
       if (__any_sync(0xffffffffu, flags & 2)) umma_commit_elect(&sh.q_empty);
-      if (++s == a.stages) {
-        s = 0;
+      if (++pair == a.pairs) {
+        pair = 0;
         ++turn;
       }
     }
     // what was issued retires before the CTA ends
-    if (scored > 0) mbar_wait(&sh.s_full[(scored - 1) & 3], ((scored - 1) >> 2) & 1, &sh.zero, kWaitNs);
+    if (scored > 0) mbar_wait(&sh.s_full[(scored - 1) & 1], ((scored - 1) >> 1) & 1, &sh.zero, kWaitNs);
   } else if (warp == 13) {
     // ---------------- output ----------------
     const uint32_t pv = idesc_16bit_f32(kBf16, 128, (heads + 15) & ~15, true, false), p_desc = desc_k(p_smem);
-    int s = 0, done = 0;
+    int pair = 0, turn = 0, done = 0;
     for (int it = 0; it < n; ++it, ++done) {
-      if (!converged_wait(sh, a.status, &sh.p_full[it & 3], it >> 2)) break;
-      const uint32_t more = (*reinterpret_cast<volatile uint32_t*>(&sh.flags[s]) & 1) ^ 1;
-      const uint32_t v_desc = desc_mn(kv_smem + s * kChunks * kBlock, kBlock), p = p_desc + (it & 1) * 64 / 16;
+      if (!converged_wait(sh, a.status, &sh.p_full[it & 1], it >> 1)) break;
+      const uint32_t more = (*reinterpret_cast<volatile uint32_t*>(&sh.flags[pair]) & 1) ^ 1;
+      const uint32_t v_desc = desc_mn(kv_smem + pair * kChunks * kBlock, kBlock);
 #pragma unroll
-      for (int t = 0; t < kOut; ++t)
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          umma_f16(tmem + t * 64, v_desc + (2 * t * kBlock + 2048 * k) / 16, p + 32 * k / 16, pv, k > 0 ? 1u : more);
-      umma_commit_elect(&sh.empty[s]);
-      umma_commit_elect(&sh.pv_done[it & 1]);
-      if (++s == a.stages) s = 0;
+        for (int t = 0; t < kOut; ++t)
+#pragma unroll
+          for (int k = 2 * half; k < 2 * half + 2; ++k)
+            umma_f16(tmem + t * 64, v_desc + (2 * t * kBlock + 2048 * k) / 16, p_desc + 32 * k / 16, pv, k > 0 ? 1u : more);
+        umma_commit_elect(&sh.empty[2 * pair + half]);
+      }
+      umma_commit_elect(&sh.pv_done);
+      if (++pair == a.pairs) {
+        pair = 0;
+        ++turn;
+      }
     }
     if (done > 0) {
-      const int last = done - 1;
-      mbar_wait(&sh.empty[last % a.stages], (last / a.stages) & 1, &sh.zero, kWaitNs);
-      mbar_wait(&sh.pv_done[last & 1], (last >> 1) & 1, &sh.zero, kWaitNs);
+      const int last = (done - 1) % a.pairs, phase = ((done - 1) / a.pairs) & 1;
+      mbar_wait(&sh.empty[2 * last], phase, &sh.zero, kWaitNs);
+      mbar_wait(&sh.empty[2 * last + 1], phase, &sh.zero, kWaitNs);
+      mbar_wait(&sh.pv_done, (done - 1) & 1, &sh.zero, kWaitNs);
     }
   } else {
     // ---------------- queries ----------------
@@ -519,7 +579,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       const char* q = static_cast<const char*>(a.q) + (at.row * a.qs0 + group * kGroup * a.qs1) * 2;
       for (int w = 0; w < 4; ++w) {
         const int hh = 16 * w + lane;
-        copy_rows<kChunks, kQBlock>(q_smem, lane < 16 && hh < heads ? q + hh * a.qs1 * 2 : nullptr, a.q, 16 * w, lane);
+        RowCopy(q_smem, lane < 16 && hh < heads ? q + hh * a.qs1 * 2 : nullptr, a.q, 16 * w, lane)
+            .template blocks<0, kChunks>();
       }
       cp_async_wait_all();
       fence_async_shared();
@@ -539,119 +600,146 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   }
 }
 
-// Joins the parts of the rows that lie in several ranges.  Block (x, h): the row
-// in which range x begins, if x is the first range to begin inside it; the parts
-// in the order of the ranges.  Range y's part is its first (slot 0) unless the
-// range begins in an earlier row (then its last, slot 1).
-template <typename T, int kLatent>
+// Joins the parts of the rows that lie in several ranges.  Grid x: the row in which
+// range x begins, if x is the first range to begin inside it; the parts in the
+// order of the ranges.  Range y's part is its first (slot 0) unless the range
+// begins in an earlier row (then its last, slot 1); a range may be empty.
+//   kWarps = 1: a warp joins one head's whole row (grid y: four heads) -- two or
+//     three parts each, many rows;
+//   kWarps = 4: the four warps of a block share the parts of one head and 128
+//     of its columns (grid z) -- a few rows spread over all ranges.
+template <typename T, int kLatent, int kWarps>
 __global__ void __launch_bounds__(128) latent_join_kernel(const __grid_constant__ LatentArgs a) {
-  __shared__ float weight[kMaxCtas];
-  __shared__ float red[8];
-  const int x = blockIdx.x + 1, h = blockIdx.y, tid = threadIdx.x;
+  constexpr int kPer = kWarps == 1 ? kLatent / 128 : 1;   // 16-byte pieces of a lane
+  const int x = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = kWarps == 1 ? static_cast<int>(blockIdx.y) * 4 + warp : static_cast<int>(blockIdx.y);
   const int64_t first = a.where[4 * x + 1], begin = a.where[4 * x + 3], before = a.where[4 * x - 1];
-  if (begin == first || before > first) return;
+  if (begin == first || before > first || h >= a.heads) return;   // kWarps = 4: the whole block
   const int64_t row = a.where[4 * x], end = first + a.where[4 * x + 2];
-  const int group = h / kGroup, hg = h % kGroup;
-  const int64_t base = ((static_cast<int64_t>(x - 1) * a.groups + group) * 2) * kGroup + hg;   // range x - 1, slot 0
   const int64_t step = static_cast<int64_t>(a.groups) * 2 * kGroup;
+  const int64_t base = (static_cast<int64_t>(x - 1) * a.groups + h / kGroup) * 2 * kGroup + h % kGroup;
   const int64_t shift = before < first ? kGroup : 0;   // range x - 1 may begin in an earlier row
-  // the parts' weights 2^(m - M); 0 for a range without tiles
+  auto part = [&](int i) { return base + i * step + (i == 0 ? shift : 0); };
   float m = -CUDART_INF_F, l = 0.0f;
   int parts = 0;
-  for (int i = tid; i < a.ranges - (x - 1); i += 128) {
+  for (int i = lane; i <= a.ranges - x; i += 32) {
     const int64_t t0 = a.where[4 * (x - 1 + i) + 3], t1 = a.where[4 * (x + i) + 3];
     if (t0 >= end) break;
     parts = i + 1;
-    if (t1 > t0) m = fmaxf(m, a.part_ml[2 * (base + i * step + (i == 0 ? shift : 0))]);
+    if (t1 > t0) m = fmaxf(m, a.part_ml[2 * part(i)]);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     parts = max(parts, __shfl_xor_sync(0xffffffffu, parts, o));
   }
-  if ((tid & 31) == 0) {
-    red[tid >> 5] = m;
-    red[4 + (tid >> 5)] = __int_as_float(parts);
-  }
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  parts = max(max(__float_as_int(red[4]), __float_as_int(red[5])), max(__float_as_int(red[6]), __float_as_int(red[7])));
   const float ref = m == -CUDART_INF_F ? 0.0f : m;
-  for (int i = tid; i < parts; i += 128) {
-    const int64_t t0 = a.where[4 * (x - 1 + i) + 3], t1 = a.where[4 * (x + i) + 3];
-    const float* ml = a.part_ml + 2 * (base + i * step + (i == 0 ? shift : 0));
-    const float w = t1 > t0 ? exp2f(ml[0] - ref) : 0.0f;
-    weight[i] = t1 > t0 ? w : -1.0f;
-    if (t1 > t0) l += ml[1] * w;
-  }
+  float4 o[kPer];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  __syncthreads();
-  if ((tid & 31) == 0) red[tid >> 5] = l;
-  __syncthreads();
-  l = (red[0] + red[1]) + (red[2] + red[3]);
-  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-  if (4 * tid < kLatent) {
-    float4 o = make_float4(0, 0, 0, 0);
-    const float* p = a.part + base * kLatent + 4 * tid;
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
-      const float w = weight[i];
-      if (w < 0.0f) continue;
-      const float4 v = *reinterpret_cast<const float4*>(p + (i * step + (i == 0 ? shift : 0)) * kLatent);
-      o = make_float4(fmaf(v.x, w, o.x), fmaf(v.y, w, o.y), fmaf(v.z, w, o.z), fmaf(v.w, w, o.w));
+  for (int c = 0; c < kPer; ++c) o[c] = make_float4(0, 0, 0, 0);
+  const int column = kWarps == 1 ? 4 * lane : static_cast<int>(blockIdx.z) * 128 + 4 * lane;
+#pragma unroll(kWarps == 1 ? 2 : 8)
+  for (int i = kWarps == 1 ? 0 : warp; i < parts; i += kWarps) {
+    if (a.where[4 * (x + i) + 3] == a.where[4 * (x - 1 + i) + 3]) continue;
+    const float w = exp2f(a.part_ml[2 * part(i)] - ref);
+    l += a.part_ml[2 * part(i) + 1] * w;
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      const float4 v = *reinterpret_cast<const float4*>(a.part + part(i) * kLatent + column + 128 * c);
+      o[c] = make_float4(fmaf(v.x, w, o[c].x), fmaf(v.y, w, o[c].y), fmaf(v.z, w, o[c].z), fmaf(v.w, w, o[c].w));
     }
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (row * a.heads + h) * kLatent + 4 * tid) =
-        make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
   }
-  if (tid == 0) a.lse[row * a.heads + h] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
+  if constexpr (kWarps == 4) {
+    __shared__ float4 sums[4][32];
+    __shared__ float ls[4];
+    sums[warp][lane] = o[0];
+    if (lane == 0) ls[warp] = l;
+    __syncthreads();
+    if (warp > 0) return;
+    l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    for (int w = 1; w < 4; ++w) {
+      const float4 v = sums[w][lane];
+      o[0] = make_float4(o[0].x + v.x, o[0].y + v.y, o[0].z + v.z, o[0].w + v.w);
+    }
+  }
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+  T* const out = static_cast<T*>(a.out) + (row * a.heads + h) * kLatent + column;
+#pragma unroll
+  for (int c = 0; c < kPer; ++c)
+    *reinterpret_cast<uint2*>(out + 128 * c) =
+        make_uint2(pack2<T>(o[c].x * inv, o[c].y * inv), pack2<T>(o[c].z * inv, o[c].w * inv));
+  if (lane == 0 && column == 0)
+    a.lse[row * a.heads + h] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
 }
 
 constexpr int64_t kMaxSmem = 232448;
 
-int64_t ranges_for(int64_t rows, int64_t heads, int64_t count) {
-  const int64_t groups = (heads + kGroup - 1) / kGroup, tiles = rows * ((count + kTile - 1) / kTile);
-  const int64_t fit = kMaxCtas / groups;
-  return tiles < fit ? (tiles > 0 ? tiles : 1) : fit;
+// How the line of tiles is cut: into `ranges` of `base` units of `unit` tiles, the
+// first `extra` ones a unit more.  Ranges that cut rows cost their parts' traffic
+// and a second launch, about as long as kJoinTiles tiles of a CTA, so rows of equal
+// length go whole to the CTAs where the longest range is not longer by more than
+// that.
+struct Cut {
+  int64_t ranges, unit, base, extra;
+  bool whole;
+};
+constexpr int64_t kJoinTiles = 6;
+
+Cut cut_for(int64_t rows, int64_t heads, int64_t count, bool equal) {
+  const int64_t fit = kMaxCtas / ((heads + kGroup - 1) / kGroup), per = (count + kTile - 1) / kTile;
+  const int64_t tiles = rows * per, ranges = tiles < fit ? (tiles > 0 ? tiles : 1) : fit;
+  Cut c{ranges, 1, tiles / ranges, tiles % ranges, false};
+  const int64_t turns = (rows + fit - 1) / fit;
+  if (equal && (ranges == 1 || turns * per <= (tiles + ranges - 1) / ranges + kJoinTiles)) {
+    c.ranges = (rows + turns - 1) / turns;
+    c = Cut{c.ranges, per, rows / c.ranges, rows % c.ranges, true};
+  }
+  return c;
 }
 
 // Launches the kernels of one element type and one pair of widths.
 template <typename T, int kLatent, int kRope>
-void launch(LatentArgs a, cudaStream_t s) {
+void launch(LatentArgs a, bool join, cudaStream_t s) {
   constexpr int kChunks = (kLatent + kRope) / 64;
-  constexpr int64_t kFixed = kChunks * kQBlock + kPBytes + 1024 + static_cast<int64_t>(sizeof(LatentShared));
-  constexpr int kStages = kFixed + 2 * kSets * kChunks * kBlock <= kMaxSmem ? 2 * kSets : kSets;
-  static_assert(kStages <= kMaxStages, "barriers");
-  constexpr int64_t kSmem = kFixed + static_cast<int64_t>(kStages) * kChunks * kBlock;
-  static_assert(kSmem <= kMaxSmem, "shared memory");
-  a.stages = kStages;
+  constexpr int64_t kFixed = (kChunks + 1) * kBlock + 1024 + static_cast<int64_t>(sizeof(LatentShared));
+  constexpr int kPairs = kFixed + 4 * kChunks * kBlock <= kMaxSmem ? 4 : 2;
+  constexpr int64_t kSmem = kFixed + static_cast<int64_t>(kPairs) * kChunks * kBlock;
+  static_assert(kPairs <= kMaxPairs && kSmem <= kMaxSmem, "shared memory");
+  a.pairs = kPairs;
   static DeviceOnce once;
   once.run([] {
     cudaFuncSetAttribute(latent_kernel<T, kLatent, kRope>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   launch_kernel_prio(LaunchPriority::kDefault, latent_kernel<T, kLatent, kRope>,
                      dim3(static_cast<unsigned>(a.ranges * a.groups)), dim3(kThreads), kSmem, s, a);
-  if (a.ranges > 1)
-    launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<T, kLatent>,
-                       dim3(static_cast<unsigned>(a.ranges - 1), static_cast<unsigned>(a.heads)), dim3(128), 0, s, a);
+  if (!join) return;
+  const unsigned cuts = static_cast<unsigned>(a.ranges - 1), heads = static_cast<unsigned>(a.heads);
+  if (a.ranges >= 8 * a.rows)
+    launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<T, kLatent, 4>, dim3(cuts, heads, kLatent / 128),
+                       dim3(128), 0, s, a);
+  else
+    launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<T, kLatent, 1>, dim3(cuts, (heads + 3) / 4),
+                       dim3(128), 0, s, a);
 }
 
 template <typename T>
-void launch_widths(const LatentArgs& a, int64_t latent, int64_t rope, cudaStream_t s) {
-  if (latent == 512) rope ? launch<T, 512, 64>(a, s) : launch<T, 512, 0>(a, s);
-  else if (latent == 384) rope ? launch<T, 384, 64>(a, s) : launch<T, 384, 0>(a, s);
-  else if (latent == 256) rope ? launch<T, 256, 64>(a, s) : launch<T, 256, 0>(a, s);
-  else rope ? launch<T, 128, 64>(a, s) : launch<T, 128, 0>(a, s);
+void launch_widths(const LatentArgs& a, int64_t latent, int64_t rope, bool join, cudaStream_t s) {
+  if (latent == 512) rope ? launch<T, 512, 64>(a, join, s) : launch<T, 512, 0>(a, join, s);
+  else if (latent == 384) rope ? launch<T, 384, 64>(a, join, s) : launch<T, 384, 0>(a, join, s);
+  else if (latent == 256) rope ? launch<T, 256, 64>(a, join, s) : launch<T, 256, 0>(a, join, s);
+  else rope ? launch<T, 128, 64>(a, join, s) : launch<T, 128, 0>(a, join, s);
 }
 
 }  // namespace
 }  // namespace v1x
 
-extern "C" int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, int64_t count, int64_t latent) {
+extern "C" int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, int64_t count, int64_t latent,
+                                                  int equal) {
   using namespace v1x;
   if (rows <= 0 || heads <= 0 || heads > 1024 || count <= 0 || latent <= 0) return 0;
-  const int64_t ranges = ranges_for(rows, heads, count), ctas = ranges * ((heads + kGroup - 1) / kGroup);
-  return (ranges + 1) * 32 + ctas * 2 * kGroup * (latent + 2) * 4;
+  const Cut c = cut_for(rows, heads, count, equal != 0);
+  if (c.whole || c.ranges == 1) return 0;
+  return (c.ranges + 1) * 32 + c.ranges * ((heads + kGroup - 1) / kGroup) * 2 * kGroup * (latent + 2) * 4;
 }
 
 extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, const void* pool, int64_t slots,
@@ -675,19 +763,22 @@ extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, con
   V1X_CHECK_ARG(!lens || (count % 64 == 0 && !req), "latent_attention: a page table takes whole pages and no slot map");
   if (rows == 0) return V1X_OK;
   V1X_CHECK_ARG(q && out && lse && (index || count == 0) && (pool || slots == 0), "latent_attention: NULL argument");
-  const int64_t need = v1x_latent_attention_workspace(rows, heads, count, latent);
+  const int64_t need = v1x_latent_attention_workspace(rows, heads, count, latent, lens == nullptr);
   V1X_CHECK_ARG(workspace_bytes >= need && (workspace || need == 0) && aligned16(workspace),
                 "latent_attention: the workspace must be 16-byte aligned and hold %lld bytes", static_cast<long long>(need));
   cudaStream_t s = as_stream(stream);
-  const int64_t groups = (heads + kGroup - 1) / kGroup, ranges = ranges_for(rows, heads, count);
+  const int64_t groups = (heads + kGroup - 1) / kGroup;
+  const Cut c = cut_for(rows, heads, count, lens == nullptr);
   LatentArgs a{q,    qs0,  qs1,   pool, slots, pool_stride, req, req_len, index, index_stride, count, lens, rows, heads,
-               0, static_cast<int>(groups), static_cast<int>(ranges), scale * kLog2e, out, lse, nullptr, nullptr, nullptr, status};
+               0, static_cast<int>(groups), static_cast<int>(c.ranges), c.unit, c.base, c.extra, scale * kLog2e, out,
+               lse, nullptr, nullptr, nullptr, status};
   if (need) {
     a.where = static_cast<int64_t*>(workspace);
-    a.part = reinterpret_cast<float*>(a.where + 4 * (ranges + 1));
-    a.part_ml = a.part + ranges * groups * 2 * kGroup * latent;
+    a.part = reinterpret_cast<float*>(a.where + 4 * (c.ranges + 1));
+    a.part_ml = a.part + c.ranges * groups * 2 * kGroup * latent;
   }
-  if (dtype == 1) launch_widths<__nv_bfloat16>(a, latent, dim - latent, s);
-  else launch_widths<__half>(a, latent, dim - latent, s);
+  V1X_CHECK_ARG(c.unit * (c.base + 1) < (int64_t(1) << 31), "latent_attention: too many tokens for one call");
+  if (dtype == 1) launch_widths<__nv_bfloat16>(a, latent, dim - latent, need > 0, s);
+  else launch_widths<__half>(a, latent, dim - latent, need > 0, s);
   return launch_status("v1x_latent_attention");
 }

@@ -85,7 +85,7 @@ def _absorbed(q, pool, request_slots, index, count, lens, scale, latent, out, ls
     out, lse = _outputs(q, (rows, heads, latent), out, lse)
     if rows == 0:
         return out, lse
-    size = _lib.lib().v1x_latent_attention_workspace(rows, heads, count, latent)
+    size = _lib.lib().v1x_latent_attention_workspace(rows, heads, count, latent, lens is None)
     work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     _lib.call("v1x_latent_attention", ptr(q), _step(q, 0), _step(q, 1), ptr(pool), pool.shape[0], _step(pool, 0),
               ptr(request_slots), 0 if request_slots is None else request_slots.shape[0], ptr(index),

@@ -647,10 +647,11 @@ V1X_API int v1x_gather_slots(const void* k, const void* v, const int32_t* req, c
  * pool_stride; out [rows, heads, latent] contiguous; dtype of q, pool and out: 1
  * bf16, 2 f16; every address and stride a multiple of 16 bytes.  latent in {128,
  * 256, 384, 512}, dim - latent in {0, 64}, heads <= 1024.  workspace: device
- * memory of at least v1x_latent_attention_workspace(...) bytes, 16-byte aligned,
- * of no meaning before or after the call (NULL if 0 bytes).  status: optional
+ * memory of at least v1x_latent_attention_workspace(rows, heads, count, latent,
+ * lens == NULL) bytes, 16-byte aligned, of no meaning before or after the call (NULL if 0 bytes).  status: optional
  * device word for V1X_STATUS_TIMEOUT. */
-V1X_API int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, int64_t count, int64_t latent);
+V1X_API int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, int64_t count, int64_t latent,
+                  int equal);
 V1X_API int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, const void* pool, int64_t slots,
                   int64_t pool_stride, const int32_t* req, int64_t req_len, const int32_t* index,
                   int64_t index_stride, int64_t count, const int32_t* lens, int64_t rows, int64_t heads,
