@@ -90,7 +90,7 @@ struct LatentShared {
   uint64_t s_full[2], p_full[2], pv_done, q_full, q_empty;
   uint64_t mask[kMaxPairs];
   uint32_t flags[kMaxPairs];   // 1: the first tile of a segment, 2: the last of a row
-  float factor[kGroup];
+  alignas(16) float factor[kGroup];
   int64_t start[4];  // as LatentArgs::where, but [3]: all tiles
   int64_t cut[2];    // base, extra
   int64_t scan[kThreads / 32 + 1];
@@ -407,41 +407,58 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
         }
         sync_128();
         T* const out = static_cast<T*>(a.out) + (static_cast<int64_t>(at.row) * a.heads + group * kGroup) * kLatent;
+        const int d = warp * 32 + lane;
+        if (whole) {
+          // 16 heads x 128 columns at a time through a half of the weights' buffer (free:
+          // the last product has read it), so that a head's 256 bytes are written as one
+          // piece; the halves alternate, one barrier a step
+          int side = 0;
 #pragma unroll 1
-        for (int t = 0; t < kOut; ++t)
+          for (int t = 0; t < kOut; ++t)
 #pragma unroll 1
-          for (int c = 0; c < cols; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(tmem + quarter + t * 64 + c, o);
-            tmem_ld_wait();
-            const int d = t * 128 + warp * 32 + lane, left = heads - c;
-            if (whole) {
-              // 32 heads x 128 columns through the weights' buffer (free: the last product
-              // has read it), so that a head's 256 bytes are written as one piece
-              uint16_t* const stage = reinterpret_cast<uint16_t*>(p_ptr) + warp * 32 + lane;
+            for (int c = 0; c < cols; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(tmem + quarter + t * 64 + c, o);
+              tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const uint32_t two = pack2<T>(__uint_as_float(o[j]) * sh.factor[c + j],
-                                              __uint_as_float(o[j + 1]) * sh.factor[c + j + 1]);
-                stage[j * 128] = static_cast<uint16_t>(two);
-                stage[(j + 1) * 128] = static_cast<uint16_t>(two >> 16);
-              }
-              sync_128();
-              T* const to = out + static_cast<int64_t>(c) * kLatent + t * 128;
+              for (int b = 0; b < 32; b += 16) {
+                uint8_t* const buffer = p_ptr + side * (kBlock / 2);
+                uint16_t* const to = reinterpret_cast<uint16_t*>(buffer) + d;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int hh = 8 * i + (tid >> 4), e = (tid & 15) * 8;
-                if (hh < left)
-                  *reinterpret_cast<uint4*>(to + hh * kLatent + e) = *reinterpret_cast<const uint4*>(p_ptr + hh * 256 + e * 2);
+                for (int j = 0; j < 16; j += 4) {
+                  const float4 f = *reinterpret_cast<const float4*>(&sh.factor[c + b + j]);
+                  const uint32_t u = pack2<T>(__uint_as_float(o[b + j]) * f.x, __uint_as_float(o[b + j + 1]) * f.y);
+                  const uint32_t v = pack2<T>(__uint_as_float(o[b + j + 2]) * f.z, __uint_as_float(o[b + j + 3]) * f.w);
+                  to[j * 128] = static_cast<uint16_t>(u);
+                  to[(j + 1) * 128] = static_cast<uint16_t>(u >> 16);
+                  to[(j + 2) * 128] = static_cast<uint16_t>(v);
+                  to[(j + 3) * 128] = static_cast<uint16_t>(v >> 16);
+                }
+                sync_128();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const int hh = 8 * i + (tid >> 4), e = (tid & 15) * 8;
+                  if (c + b + hh < heads)
+                    *reinterpret_cast<uint4*>(out + (c + b + hh) * kLatent + t * 128 + e) =
+                        *reinterpret_cast<const uint4*>(buffer + hh * 256 + e * 2);
+                }
+                side ^= 1;
               }
-              sync_128();
-            } else {
-              float* const to = part + c * kLatent + d;
+            }
+        } else {
+#pragma unroll 1
+          for (int t = 0; t < kOut; ++t)
+#pragma unroll 1
+            for (int c = 0; c < cols; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(tmem + quarter + t * 64 + c, o);
+              tmem_ld_wait();
+              float* const to = part + c * kLatent + t * 128 + d;
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (j < left) to[j * kLatent] = __uint_as_float(o[j]);
+                if (c + j < heads) to[j * kLatent] = __uint_as_float(o[j]);
             }
-          }
+        }
         tc_fence_before();
         sync_128();                              // factor is free again
         ++segment;
