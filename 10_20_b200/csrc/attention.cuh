@@ -24,6 +24,12 @@ __device__ __forceinline__ float2 to_float2<__half>(uint32_t two) {
   return __half22float2(*reinterpret_cast<__half2*>(&two));
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // two floats rounded to nearest even, the first in the low half
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);

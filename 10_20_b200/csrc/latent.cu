@@ -137,12 +137,6 @@ __device__ __forceinline__ int64_t range_start(int64_t x, int64_t unit, int64_t 
   return (x * base + min(x, extra)) * unit;
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ void give_up(LatentShared& sh, int32_t* status) {
   *reinterpret_cast<volatile int*>(&sh.abort) = 1;
   if (status) atomicExch(status, V1X_STATUS_TIMEOUT);
@@ -486,10 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     };
     int64_t slot = turn_of < n ? slot_ahead() : -1;
     for (int it = turn_of; it < n; it += 2) {
-      if (!mbar_wait(&sh.empty[2 * pair + half], (turn & 1) ^ 1, &sh.abort, kWaitNs)) {
-        give_up(sh, a.status);
-        break;
-      }
+      if (!converged_wait(sh, a.status, &sh.empty[2 * pair + half], turn ^ 1)) break;
       const unsigned some = __ballot_sync(0xffffffffu, slot >= 0) & 0xFFFFu;
       if (lane == 0) {
         reinterpret_cast<volatile uint16_t*>(&sh.mask[pair])[R0 >> 4] = static_cast<uint16_t>(some);
@@ -589,10 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     // ---------------- queries ----------------
     int rows_loaded = 0;
     for (int it = 0; it < n;) {
-      if (!mbar_wait(&sh.q_empty, (rows_loaded & 1) ^ 1, &sh.abort, kWaitNs)) {
-        give_up(sh, a.status);
-        break;
-      }
+      if (!converged_wait(sh, a.status, &sh.q_empty, rows_loaded ^ 1)) break;
       const char* q = static_cast<const char*>(a.q) + (at.row * a.qs0 + group * kGroup * a.qs1) * 2;
       for (int w = 0; w < 4; ++w) {
         const int hh = 16 * w + lane;

@@ -1,77 +1,415 @@
-// Latent attention, expanded form: see v1x_prompt_attention in v1x.h.
+// Latent attention, expanded form, on the tensor cores: see v1x_prompt_attention
+// in v1x.h.
 //
-// One warp per (query, head), one key per step: the query, the running maximum
-// and sum of the softmax (in powers of two) and the output row in registers.
+// A CTA has 256 queries of one request and head, two tiles of 128, and goes over
+// the keys that they see in tiles of 128:
+//
+//   S_t[128 x 128]  = Q_t . [K | K_rope]^T    K = 128 + dr, operands in shared memory
+//   O_t[128 x 128] += P_t . V                 P in TMEM, over S_t
+//
+// One query per TMEM lane: a softmax thread owns a query's row, so maxima, sums and
+// the rescale of O need no exchange.  The running maximum that the weights are taken
+// against moves only when a tile exceeds it by more than 2^8, so that O is rescaled
+// a few times a row at most; sums stay in 32 bits, the weights are rounded once, to
+// the inputs' type, for the second product.
+//
+// The tensor cores alternate between the tiles (S_0, O_1, S_1, O_0, ...), so that one
+// tile's softmax runs beside the other's products: 2560 cycles of MMA per 128 keys
+// with dr = 64 against 2048 of exp2 for both tiles, at the hardware's rates.
+// 96 KB of queries leave room for three 32 KB slots that keys and values take in
+// turn and two 16 KB slots of rotary keys; the rows come by 16-byte cp.async, which
+// takes any strides and writes zeros past the request's last key (a neighbour's
+// values never enter a product).
+//
+// Warp roles (384 threads, one CTA per SM): 0-3 and 4-7 softmax and epilogue of the
+// two tiles, 8 TMEM owner and MMA issuer, 9-10 keys and values (64 rows each), 11
+// the queries, then the rotary keys.  Later queries see more keys: the grid begins
+// with the last ones, all heads of a tile side by side.
+// Waits are bounded (2 s, then V1X_STATUS_TIMEOUT).
+#include <type_traits>
+
 #include "attention.cuh"
+#include "sm100.cuh"
 
 namespace v1x {
 namespace {
 
 using namespace attn;
+using namespace sm100;
+
+constexpr int kRows = 128;                // queries of a tile, keys of a tile
+constexpr int kBlock = kRows * 128;       // bytes of 64 elements of a tile's rows
+constexpr int kThreads = 384;
+constexpr int kSlots = 3, kRopeSlots = 2;
+constexpr uint32_t kOutCol = 256;         // TMEM: S_0, S_1 in columns 0-255 (P over them), O_0, O_1
+constexpr float kLazy = 8.0f;             // log2 of the growth that the weights may show before a rescale
+constexpr uint64_t kWaitNs = 2000000000ull;
 
 struct PromptArgs {
   const void *q, *k, *k_rope, *v;
   int64_t qs0, qs1, ks0, ks1, krs0, vs0, vs1;
   const int32_t *offsets, *kv_offsets;
   int64_t requests, tokens, keys, heads;
-  int dr;
-  float scale_log2;
+  float scale_log2;      // of |scale|
+  int negative;          // the scale's sign goes into the product
   void* out;
   float* lse;
+  int32_t* status;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(128) prompt_rows_kernel(const __grid_constant__ PromptArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t i = blockIdx.x, h = static_cast<int64_t>(blockIdx.y) * 4 + (threadIdx.x >> 5);
-  if (h >= a.heads) return;
-  // the last request whose first query is at or before i
-  int64_t lo = 0, hi = a.requests;
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (a.offsets[mid] <= i) lo = mid;
-    else hi = mid;
+struct PromptShared {
+  uint64_t full[kSlots], empty[kSlots], rope_full[kRopeSlots], rope_empty[kRopeSlots];
+  uint64_t q_full, s_full[2], p_full[2], pv_done[2], o_done;
+  int64_t request;
+  uint32_t tmem;
+  int abort, zero;
+};
+
+__device__ __forceinline__ void give_up(PromptShared& sh, int32_t* status) {
+  *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+  if (status) atomicExch(status, V1X_STATUS_TIMEOUT);
+}
+
+__device__ __forceinline__ bool converged_wait(PromptShared& sh, int32_t* status, uint64_t* bar, int phase) {
+  const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, &sh.abort, kWaitNs));
+  if (!ok) give_up(sh, status);
+  tc_fence_after();
+  return ok;
+}
+
+__device__ __forceinline__ int64_t clamped(const int32_t* offsets, int64_t i, int64_t most) {
+  return min(static_cast<int64_t>(max(offsets[i], 0)), most);
+}
+
+// `kCount` rows of kBlocks x 64 elements from row `row` on, into the swizzled operand
+// layout (row R of block b at b * kBlock + R * 128, its 16-byte pieces permuted by
+// R & 7); rows from `rows` on become zeros.  A warp moves four rows' 128-byte pieces
+// at a time.
+template <int kBlocks, int kCount>
+__device__ __forceinline__ void copy_tile(uint32_t dst, int R0, const char* src, int64_t stride, int64_t row, int64_t rows,
+                                          const void* any, int lane) {
+  const int r = lane >> 3, piece = lane & 7;
+  const char* p = src + (row + r) * stride + piece * 16;
+#pragma unroll 4
+  for (int i = 0; i < kCount; i += 4, p += 4 * stride) {
+    const int R = R0 + i + r;
+    const bool live = row + i + r < rows;
+    const uint32_t to = dst + R * 128 + ((piece ^ (R & 7)) << 4);
+    const char* const from = live ? p : static_cast<const char*>(any);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) cp_async16(to + b * kBlock, from + (live ? b * 128 : 0), live ? 16 : 0);
   }
-  const int64_t q0 = max(a.offsets[lo], 0), q1 = min(static_cast<int64_t>(a.offsets[lo + 1]), a.tokens);
-  if (i < q0 || i >= q1) return;
-  const int64_t k0 = max(a.kv_offsets[lo], 0), k1 = min(static_cast<int64_t>(a.kv_offsets[lo + 1]), a.keys);
-  const int64_t end = min(k1, k0 + (i - q0) + 1 + (k1 - k0) - (q1 - q0));
-  const T* q = static_cast<const T*>(a.q) + i * a.qs0 + h * a.qs1;
-  float2 qv[3];
-#pragma unroll
-  for (int c = 0; c < 3; ++c)
-    qv[c] = c < 2 || a.dr ? to_float2<T>(*reinterpret_cast<const uint32_t*>(q + 64 * c + 2 * lane)) : make_float2(0, 0);
-  float2 acc[2] = {make_float2(0, 0), make_float2(0, 0)};
-  float m = -CUDART_INF_F, l = 0.0f;
-  for (int64_t j = k0; j < end; ++j) {
-    const T* k = static_cast<const T*>(a.k) + j * a.ks0 + h * a.ks1 + 2 * lane;
-    const T* v = static_cast<const T*>(a.v) + j * a.vs0 + h * a.vs1 + 2 * lane;
-    float dot = 0.0f;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float2 x = to_float2<T>(*reinterpret_cast<const uint32_t*>(k + 64 * c));
-      dot = fmaf(qv[c].x, x.x, fmaf(qv[c].y, x.y, dot));
+}
+
+template <typename T, bool kRope>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs a) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kQBlocks = kRope ? 3 : 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t q_smem = smem_u32(base), kv_smem = q_smem + 6 * kBlock, rope_smem = kv_smem + kSlots * 2 * kBlock;
+  PromptShared& sh = *reinterpret_cast<PromptShared*>(base + (6 + 2 * kSlots + kRopeSlots) * kBlock);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t h = blockIdx.x, unit = static_cast<int64_t>(gridDim.y) - 1 - blockIdx.y;
+
+  // ---- the unit's request: the last one with offsets[r] / 256 + r <= unit; a request
+  // has at least as many units as tiles of 256 queries ------------------------------
+  if (warp == 0) {
+    int64_t lo = 0, n = a.requests;
+    while (n > 1) {
+      const int64_t step = (n + 31) / 32, c = lo + lane * step;
+      const bool at = lane * step < n && clamped(a.offsets, c, a.tokens) / 256 + c <= unit;
+      const int64_t k = max(__popc(__ballot_sync(0xffffffffu, at)) - 1, 0);
+      lo += k * step;
+      n = min(step, n - k * step);
     }
-    if (a.dr) {
-      const float2 x = to_float2<T>(*reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.k_rope) + j * a.krs0 + 2 * lane));
-      dot = fmaf(qv[2].x, x.x, fmaf(qv[2].y, x.y, dot));
+    if (lane == 0) sh.request = lo;
+  }
+  __syncthreads();
+  const int64_t r = sh.request;
+  const int64_t q0 = clamped(a.offsets, r, a.tokens), q1 = max(clamped(a.offsets, r + 1, a.tokens), q0);
+  const int64_t k0 = clamped(a.kv_offsets, r, a.keys), k1 = max(clamped(a.kv_offsets, r + 1, a.keys), k0);
+  const int64_t nq = q1 - q0, nk = k1 - k0, tile = unit - (q0 / 256 + r);
+  const int64_t i0 = tile * 256;                           // the first query of the request in this CTA
+  if (tile < 0 || i0 >= nq) return;
+  // key tiles that a tile of queries sees: up to its last query's limit
+  auto tiles_seen = [&](int t) {
+    const int64_t last = min(i0 + 128 * (t + 1), nq) - 1;
+    if (last < i0 + 128 * t) return 0;
+    const int64_t limit = min(last + 1 + nk - nq, nk);
+    return limit > 0 ? static_cast<int>((limit + kRows - 1) / kRows) : 0;
+  };
+  const int n0 = tiles_seen(0), n1 = tiles_seen(1), n = max(n0, n1);
+
+  if (tid == 0) {
+    sh.abort = 0;
+    sh.zero = 0;
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&sh.full[i], 2);
+      mbar_init(&sh.empty[i], 1);
     }
-    const float x = warp_sum(dot) * a.scale_log2, top = fmaxf(m, x);
-    const float shrink = exp2f(m - top), p = exp2f(x - top);
-    l = l * shrink + p;
-    m = top;
+    for (int i = 0; i < kRopeSlots; ++i) {
+      mbar_init(&sh.rope_full[i], 1);
+      mbar_init(&sh.rope_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.pv_done[i], 1);
+    }
+    mbar_init(&sh.q_full, 1);
+    mbar_init(&sh.o_done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < 8) {
+    // ---------------- softmax, rescale, epilogue ----------------
+    const int t = warp >> 2;
+    const int64_t i = i0 + 128 * t + 32 * (warp & 3) + lane;     // the thread's query of the request
+    const int64_t limit = i < nq ? max(min(i + 1 + nk - nq, nk), static_cast<int64_t>(0)) : 0;
+    const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + quarter + 128 * t, o_addr = tmem + quarter + kOutCol + 128 * t;
+    const int mine = t ? n1 : n0;
+    const float c = a.scale_log2;
+    float m = -CUDART_INF_F, l = 0.0f;       // m: of the unscaled scores
+    bool ok = true;
+    for (int j = 0; j < mine; ++j) {
+      if (ok && !mbar_wait(&sh.s_full[t], j & 1, &sh.abort, kWaitNs)) {
+        give_up(sh, a.status);
+        ok = false;
+      }
+      if (__any_sync(0xffffffffu, !ok)) break;
+      tc_fence_after();
+      uint32_t s[4][32];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float2 y = to_float2<T>(*reinterpret_cast<const uint32_t*>(v + 64 * c));
-      acc[c].x = fmaf(p, y.x, acc[c].x * shrink);
-      acc[c].y = fmaf(p, y.y, acc[c].y * shrink);
+      for (int b = 0; b < 4; ++b) tmem_ld32(s_addr + 32 * b, s[b]);
+      tmem_ld_wait();
+      if (__any_sync(0xffffffffu, limit < static_cast<int64_t>(j + 1) * kRows)) {
+        const int left = static_cast<int>(max(min(limit - static_cast<int64_t>(j) * kRows, static_cast<int64_t>(kRows)),
+                                              static_cast<int64_t>(0)));
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (32 * b + e >= left) s[b][e] = 0xFF800000u;   // -inf
+      }
+      float top[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        top[b] = __uint_as_float(s[b][0]);
+#pragma unroll
+        for (int e = 1; e < 32; ++e) top[b] = fmaxf(top[b], __uint_as_float(s[b][e]));
+      }
+      const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if (j == 0) {
+        m = most;
+      } else {
+        // s_full says that every product issued before is complete, O's included
+        const bool grows = m == -CUDART_INF_F ? most > m : (most - m) * c > kLazy;
+        if (__any_sync(0xffffffffu, grows)) {
+          const float f = grows ? (m == -CUDART_INF_F ? 0.0f : exp2_fast((m - most) * c)) : 1.0f;
+          if (grows) m = most;
+          l *= f;
+#pragma unroll 1
+          for (int b = 0; b < 4; ++b) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + 32 * b, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st32(o_addr + 32 * b, o);
+          }
+        }
+      }
+      const float shift = m == -CUDART_INF_F ? 0.0f : -m * c;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          const float u = exp2_fast(fmaf(__uint_as_float(s[2 * half + (e >> 5)][e & 31]), c, shift));
+          const float v = exp2_fast(fmaf(__uint_as_float(s[2 * half + (e >> 5)][(e & 31) + 1]), c, shift));
+          sum[(e >> 1) & 3] += u + v;
+          w[e >> 1] = pack2<T>(u, v);
+        }
+        tmem_st32(s_addr + 32 * half, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[t]);
+    }
+    if (mine > 0 && ok && !mbar_wait(&sh.o_done, 0, &sh.abort, kWaitNs)) give_up(sh, a.status);
+    __syncwarp();
+    tc_fence_after();
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    T* const out = static_cast<T*>(a.out) + ((q0 + i) * a.heads + h) * 128;
+#pragma unroll 1
+    for (int b = 0; b < 4; ++b) {
+      uint32_t o[32];
+      if (mine > 0) {
+        tmem_ld32(o_addr + 32 * b, o);
+        tmem_ld_wait();
+      }
+      if (i < nq) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            w[x] = l == 0.0f ? 0u
+                             : pack2<T>(__uint_as_float(o[e + 2 * x]) * inv, __uint_as_float(o[e + 2 * x + 1]) * inv);
+          *reinterpret_cast<uint4*>(out + 32 * b + e) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+    if (i < nq)
+      a.lse[(q0 + i) * a.heads + h] = l > 0.0f ? (m * c + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
+    tc_fence_before();
+  } else if (warp == 8) {
+    // ---------------- MMA issuer ----------------
+    if (n > 0) {
+      const uint32_t qk = idesc_16bit_f32(kBf16, 128, 128, false, false) | (a.negative ? 1u << 13 : 0u);
+      const uint32_t pv = idesc_16bit_f32(kBf16, 128, 128, false, true);
+      bool ok = converged_wait(sh, a.status, &sh.q_full, 0);
+      int issued = 0;
+      auto scores = [&](int t, int j) {
+        const int u = 2 * j, slot = u % kSlots, rope = j % kRopeSlots;
+        const bool last = t == 1 || j >= n1;
+        ok = ok && converged_wait(sh, a.status, &sh.full[slot], u / kSlots);
+        if (kRope) ok = ok && converged_wait(sh, a.status, &sh.rope_full[rope], j / kRopeSlots);
+        if (j > 0) ok = ok && converged_wait(sh, a.status, &sh.pv_done[t], j - 1);   // P_t is read: S_t may be written
+        if (!ok) return;
+        const uint32_t qd = desc_k(q_smem + t * kQBlocks * kBlock), kd = desc_k(kv_smem + slot * 2 * kBlock);
+        const uint32_t rd = desc_k(rope_smem + rope * kBlock), d = tmem + 128 * t;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(d, qd + (b * kBlock + 32 * k) / 16, kd + (b * kBlock + 32 * k) / 16, qk, b + k > 0 ? 1u : 0u);
+        if (kRope) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_f16(d, qd + (2 * kBlock + 32 * k) / 16, rd + 32 * k / 16, qk, 1u);
+        }
+        umma_commit_elect(&sh.s_full[t]);
+        if (last) {
+          umma_commit_elect(&sh.empty[slot]);
+          if (kRope) umma_commit_elect(&sh.rope_empty[rope]);
+        }
+        issued = 1;
+      };
+      auto output = [&](int t, int j) {
+        const int u = 2 * j + 1, slot = u % kSlots;
+        const bool last = t == 1 || j >= n1;
+        ok = ok && converged_wait(sh, a.status, &sh.full[slot], u / kSlots);
+        ok = ok && converged_wait(sh, a.status, &sh.p_full[t], j);
+        if (!ok) return;
+        const uint32_t vd = desc_mn(kv_smem + slot * 2 * kBlock, kBlock), d = tmem + kOutCol + 128 * t, p = tmem + 128 * t;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) umma_f16_ta(d, p + 8 * k, vd + 2048 * k / 16, pv, j + k > 0 ? 1u : 0u);
+        umma_commit_elect(&sh.pv_done[t]);
+        if (last) umma_commit_elect(&sh.empty[slot]);
+      };
+      if (n0 > 0) scores(0, 0);
+      if (n1 > 0) scores(1, 0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j < n0) {
+          output(0, j);
+          if (j + 1 < n0) scores(0, j + 1);
+        }
+        if (j < n1) {
+          output(1, j);
+          if (j + 1 < n1) scores(1, j + 1);
+        }
+      }
+      // everything that was issued retires before the CTA ends
+      if (issued) {
+        umma_commit_elect(&sh.o_done);
+        mbar_wait(&sh.o_done, 0, &sh.zero, kWaitNs);
+      }
+    }
+  } else if (warp < 11) {
+    // ---------------- keys and values ----------------
+    const int half = warp - 9;
+    const char* const k = static_cast<const char*>(a.k) + (k0 * a.ks0 + h * a.ks1) * 2;
+    const char* const v = static_cast<const char*>(a.v) + (k0 * a.vs0 + h * a.vs1) * 2;
+    int pending = -1;                            // a load whose arrival has not been reported
+    auto report = [&] {
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.full[pending % kSlots]);
+    };
+    for (int u = 0; u < 2 * n; ++u) {
+      const int slot = u % kSlots, phase = ((u / kSlots) & 1) ^ 1;
+      if (pending >= 0 && !__all_sync(0xffffffffu, mbar_test(&sh.empty[slot], phase))) {
+        cp_async_wait<0>();
+        report();
+        pending = -1;
+      }
+      if (!converged_wait(sh, a.status, &sh.empty[slot], phase)) break;
+      const int64_t row = static_cast<int64_t>(u >> 1) * kRows + 64 * half;
+      copy_tile<2, 64>(kv_smem + slot * 2 * kBlock, 64 * half, u & 1 ? v : k, (u & 1 ? a.vs0 : a.ks0) * 2, row, nk, a.q, lane);
+      cp_async_commit();
+      if (pending >= 0) {
+        cp_async_wait<1>();
+        report();
+      }
+      pending = u;
+    }
+    cp_async_wait_all();
+    if (pending >= 0) report();
+  } else {
+    // ---------------- queries, rotary keys ----------------
+    if (n > 0) {
+      const char* const q = static_cast<const char*>(a.q) + (q0 * a.qs0 + h * a.qs1) * 2;
+      for (int t = 0; t < 2; ++t)
+        copy_tile<kQBlocks, 128>(q_smem + t * kQBlocks * kBlock, 0, q, a.qs0 * 2, i0 + 128 * t, nq, a.q, lane);
+      cp_async_wait_all();
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full);
+      if (kRope) {
+        const char* const kr = static_cast<const char*>(a.k_rope) + k0 * a.krs0 * 2;
+        for (int j = 0; j < n; ++j) {
+          const int slot = j % kRopeSlots;
+          if (!converged_wait(sh, a.status, &sh.rope_empty[slot], (j / kRopeSlots) ^ 1)) break;
+          copy_tile<1, 128>(rope_smem + slot * kBlock, 0, kr, a.krs0 * 2, static_cast<int64_t>(j) * kRows, nk, a.q, lane);
+          cp_async_wait_all();
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.rope_full[slot]);
+        }
+        cp_async_wait_all();
+      }
     }
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  T* out = static_cast<T*>(a.out) + (i * a.heads + h) * 128 + 2 * lane;
-#pragma unroll
-  for (int c = 0; c < 2; ++c) *reinterpret_cast<uint32_t*>(out + 64 * c) = pack2<T>(acc[c].x * inv, acc[c].y * inv);
-  if (lane == 0) a.lse[i * a.heads + h] = l > 0.0f ? (m + log2f(l)) * kLn2 : -CUDART_INF_F;
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+constexpr int kSmem = 1024 + (6 + 2 * kSlots + kRopeSlots) * kBlock + static_cast<int>(sizeof(PromptShared));
+static_assert(kSmem <= 232448, "shared memory");
+
+template <typename T, bool kRope>
+void launch(const PromptArgs& a, cudaStream_t s) {
+  static DeviceOnce once;
+  once.run([] { cudaFuncSetAttribute(prompt_kernel<T, kRope>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem); });
+  launch_kernel_prio(LaunchPriority::kDefault, prompt_kernel<T, kRope>,
+                     dim3(static_cast<unsigned>(a.heads), static_cast<unsigned>(a.tokens / 256 + a.requests)),
+                     dim3(kThreads), kSmem, s, a);
 }
 
 }  // namespace
@@ -89,6 +427,7 @@ extern "C" int v1x_prompt_attention(const void* q, int64_t qs0, int64_t qs1, con
   V1X_CHECK_ARG(tokens >= 0 && tokens < (int64_t(1) << 31) && keys >= 0 && keys < (int64_t(1) << 31) && requests >= 0 &&
                     heads >= 1 && heads <= 1024,
                 "prompt_attention: bad geometry");
+  V1X_CHECK_ARG(tokens / 256 + requests <= 65535, "prompt_attention: at most 65535 tiles of 256 queries and requests");
   V1X_CHECK_ARG((dr == 0 && !k_rope) || (dr == 64 && (k_rope || keys == 0)), "prompt_attention: dr must be 0 without k_rope, 64 with it");
   V1X_CHECK_ARG(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(k_rope) |
                   reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
@@ -96,12 +435,12 @@ extern "C" int v1x_prompt_attention(const void* q, int64_t qs0, int64_t qs1, con
                 "prompt_attention: q, k, k_rope, v and out rows must be 16-byte aligned");
   if (tokens == 0 || requests == 0) return V1X_OK;
   V1X_CHECK_ARG(q && out && lse && offsets && kv_offsets && ((k && v) || keys == 0), "prompt_attention: NULL argument");
-  PromptArgs a{q,   k,   k_rope, v,   qs0, qs1, ks0, ks1, krs0, vs0, vs1, offsets, kv_offsets, requests, tokens,
-               keys, heads, static_cast<int>(dr), scale * kLog2e, out, lse};
-  const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>((heads + 3) / 4));
-  if (dtype == 1)
-    launch_kernel_prio(LaunchPriority::kDefault, prompt_rows_kernel<__nv_bfloat16>, grid, dim3(128), 0, as_stream(stream), a);
-  else
-    launch_kernel_prio(LaunchPriority::kDefault, prompt_rows_kernel<__half>, grid, dim3(128), 0, as_stream(stream), a);
+  // a masked score, -inf, has to stay -inf under the scale
+  const float magnitude = scale == 0 ? 1e-30f : (scale < 0 ? -scale : scale) * kLog2e;
+  const PromptArgs a{q,    k,     k_rope, v, qs0, qs1, ks0, ks1, krs0, vs0, vs1, offsets, kv_offsets, requests, tokens,
+                     keys, heads, magnitude, scale < 0 ? 1 : 0, out, lse, status};
+  cudaStream_t s = as_stream(stream);
+  if (dtype == 1) dr ? launch<__nv_bfloat16, true>(a, s) : launch<__nv_bfloat16, false>(a, s);
+  else dr ? launch<__half, true>(a, s) : launch<__half, false>(a, s);
   return launch_status("v1x_prompt_attention");
 }

@@ -247,6 +247,15 @@ def test_prompt(counts, extra, heads, rope, dtype):
     check(out, lse, want_prompt(q, k, kr, v, qo, ko, 0.08, dtype))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.05, 0.9])
+def test_prompt_scales(scale):
+    """Equal weights, the reversed order, and rows where the maximum keeps moving far."""
+    q, kv, kr = normal((300, 2, 192), "bf16", 41), normal((420, 2, 256), "bf16", 42), normal((420, 64), "bf16", 43)
+    kv[:, 0, :128] *= torch.linspace(0.0, 3.0, 420, device=DEV)[:, None].to(torch.bfloat16)
+    out, lse = L.attend_prompt(q, kv[..., :128], kr, kv[..., 128:], ints([0, 300]), scale, kv_offsets=ints([0, 420]))
+    check(out, lse, want_prompt(q, kv[..., :128], kr, kv[..., 128:], [0, 300], [0, 420], scale, "bf16"))
+
+
 def test_prompt_poison_and_uncovered_rows():
     """NaN and infinities in the keys of nobody; rows of q outside every request stay as they were."""
     q, kv, kr = normal((400, 2, 192), "bf16", 33), normal((900, 2, 256), "bf16", 34), normal((900, 64), "bf16", 35)
