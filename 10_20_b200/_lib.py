@@ -77,7 +77,7 @@ SIGNATURES = {
                              P, P, P],
     "v1x_kv8_store": [P, P, P, P, I64, I64, P, I64, I64, P, I64, I64, I32, I64, P, I64, I64, P, P, I64, P],
     "v1x_kv8_attend_workspace": [I64, I64, I64, I64],
-    "v1x_kv8_attend": [P, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P, I64, I64, F32, I32, P, P, P, I64, P],
+    "v1x_kv8_attend": [P, I64, I64, P, P, P, P, I64, I64, P, I64, I64, P, I64, I64, F32, I32, P, P, P, I64, P, P],
     "v1x_build_workspace_bytes": [I64],
     "v1x_build_buckets": [P, I64, P, P, P, P, P, P, P, P, I64, P],
     "v1x_build_buckets_noalloc": [P, I64, P, P, P, P, P, P, P, I64, P],

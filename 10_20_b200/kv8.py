@@ -93,6 +93,6 @@ def attend(q, k_cache, k_scale, v_cache, v_scale, table, lens, scale, out=None, 
     work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     _lib.call("v1x_kv8_attend", ptr(q), _step(q, 0), _step(q, 1), ptr(k_cache), ptr(k_scale), ptr(v_cache),
               ptr(v_scale), pages, kv_heads, ptr(table), _step(table, 0), table.shape[1], ptr(lens), rows, heads,
-              float(scale), _DTYPES[q.dtype], ptr(out), ptr(lse), ptr(work), size, _lib.stream_of(q),
+              float(scale), _DTYPES[q.dtype], ptr(out), ptr(lse), ptr(work), size, None, _lib.stream_of(q),
               device=q.device)
     return out, lse

@@ -131,12 +131,15 @@ def test_entry_points_refuse_before_a_launch():
     lib = importlib.import_module("10_20_b200._lib").lib()
     x = 1 << 20   # an aligned address that is never read
 
-    def latent(dtype=1, q=x, qs=576, heads=4, dim=576, latent=512, count=64, lens=None, index=x, req=None):
-        return lib.v1x_latent_attention(q, qs * heads, qs, x, 64, 576, req, 8, index, count, count, lens, 2, heads, dim,
-                                        latent, 0.1, dtype, x, x, None, 0, None, None)
+    def latent(dtype=1, q=x, qs=576, heads=4, dim=576, latent=512, count=64, lens=None, index=x, req=None, rows=2,
+               work=x, size=1 << 30):
+        return lib.v1x_latent_attention(q, qs * heads, qs, x, 64, 576, req, 8, index, count, count, lens, rows, heads, dim,
+                                        latent, 0.1, dtype, x, x, work, size, None, None)
 
     for bad in (dict(dtype=0), dict(q=x + 2), dict(qs=577), dict(heads=0), dict(heads=1025), dict(dim=560),
-                dict(latent=64, dim=64), dict(count=65, lens=x), dict(lens=x, req=x), dict(index=None), dict(q=None)):
+                dict(latent=64, dim=64), dict(count=65, lens=x), dict(lens=x, req=x), dict(index=None), dict(q=None),
+                dict(rows=1, count=65536, size=0), dict(rows=1, count=65536, work=x + 8),
+                dict(rows=1 << 30, count=1 << 35)):
         assert latent(**bad) == -1, bad
         assert b"latent_attention" in lib.v1x_last_error()
     pr = [x, 768, 192, x, 512, 128, x, 64, x, 512, 128, x, x, 1, 8, 8, 4, 64, 0.1, 1, x, x, None, None]
@@ -151,8 +154,8 @@ def test_entry_points_refuse_before_a_launch():
         bad[at] = v
         assert lib.v1x_kv8_store(*bad) == -1, (at, v)
         assert b"kv8_store" in lib.v1x_last_error()
-    at_ = [x, 512, 128, x, x, x, x, 4, 2, x, 2, 2, x, 1, 4, 0.1, 1, x, x, None, 0, None]
-    for at, v in ((16, 0), (14, 3), (0, x + 2), (1, 511), (12, None), (9, None), (17, None)):
+    at_ = [x, 512, 128, x, x, x, x, 4, 2, x, 2, 2, x, 1, 4, 0.1, 1, x, x, x, 1 << 30, None, None]
+    for at, v in ((16, 0), (14, 3), (0, x + 2), (1, 511), (12, None), (9, None), (17, None), (20, 0), (19, x + 8), (7, 1 << 25)):
         bad = list(at_)
         bad[at] = v
         assert lib.v1x_kv8_attend(*bad) == -1, (at, v)
