@@ -20,24 +20,32 @@ as ``latent_attention`` does.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
 
 from . import _lib
 from ._lib import ptr, require
-from .latent_attention import PAGE, _DTYPES, _index, _outputs, _rows16, _step
+from .latent_attention import PAGE, _DTYPES, _index, _one_device, _outputs, _rows16, _step
 
 
 def _cache(k_cache, k_scale, v_cache, v_scale):
-    require(k_cache.dim() == 4 and k_cache.shape[2:] == (PAGE, 128) and v_cache.shape == k_cache.shape
-            and k_cache.shape[1] >= 1,
+    shape = k_cache.shape
+    require(len(shape) == 4 and shape[2:] == (PAGE, 128) and v_cache.shape == shape and shape[1] >= 1,
             "k_cache, v_cache: [pages, kv_heads, 64, 128]")
-    require(all(t.dtype == torch.float8_e4m3fn and t.is_contiguous() and t.data_ptr() % 16 == 0
-                for t in (k_cache, v_cache)), "k_cache, v_cache: contiguous float8_e4m3fn, 16-byte aligned")
-    require(all(t.shape == k_cache.shape[:2] and t.dtype == torch.float32 and t.is_contiguous()
-                for t in (k_scale, v_scale)), "k_scale, v_scale: contiguous float32 [pages, kv_heads]")
-    return k_cache.shape[0], k_cache.shape[1]
+    require(k_cache.dtype is torch.float8_e4m3fn and v_cache.dtype is torch.float8_e4m3fn and k_cache.is_contiguous()
+            and v_cache.is_contiguous() and k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0,
+            "k_cache, v_cache: contiguous float8_e4m3fn, 16-byte aligned")
+    require(k_scale.shape == shape[:2] and v_scale.shape == shape[:2] and k_scale.dtype is torch.float32
+            and v_scale.dtype is torch.float32 and k_scale.is_contiguous() and v_scale.is_contiguous(),
+            "k_scale, v_scale: contiguous float32 [pages, kv_heads]")
+    return shape[0], shape[1]
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(rows, heads, kv_heads, table_pages) -> int:
+    return _lib.lib().v1x_kv8_attend_workspace(rows, heads, kv_heads, table_pages)
 
 
 def store(k_cache, k_scale, v_cache, v_scale, k, v, table, prefix, offsets):
@@ -51,23 +59,25 @@ def store(k_cache, k_scale, v_cache, v_scale, k, v, table, prefix, offsets):
     are.  No two requests of a call may write the same page.  Storing the same
     tokens again changes nothing."""
     pages, heads = _cache(k_cache, k_scale, v_cache, v_scale)
-    require(k.dim() == 3 and k.shape[1:] == (heads, 128) and v.shape == k.shape and k.dtype == v.dtype
-            and k.dtype in _DTYPES, f"k, v: [tokens, {heads}, 128], both bfloat16 or both float16")
+    code = _DTYPES.get(k.dtype)
+    require(k.dim() == 3 and k.shape[1:] == (heads, 128) and v.shape == k.shape and k.dtype is v.dtype
+            and code is not None, "k, v: [tokens, kv_heads, 128], both bfloat16 or both float16")
     require(_rows16(k) and _rows16(v), "k, v: unit inner stride, rows 16-byte aligned")
-    require(prefix.dtype == torch.int32 and prefix.dim() == 1 and prefix.is_contiguous(),
+    require(prefix.dtype is torch.int32 and prefix.dim() == 1 and prefix.is_contiguous(),
             "prefix: contiguous int32 [requests]")
     requests = prefix.shape[0]
-    require(offsets.dtype == torch.int32 and offsets.shape == (requests + 1,) and offsets.is_contiguous(),
+    require(offsets.dtype is torch.int32 and offsets.shape == (requests + 1,) and offsets.is_contiguous(),
             "offsets: contiguous int32 [requests + 1]")
     require(_index(table, requests), "table: int32 [requests, pages] with unit inner stride")
     require(k.is_cuda, "k must be a CUDA tensor (there is no CPU path)")
-    _lib.same_device(k_cache, k_scale, v_cache, v_scale, k, v, table, prefix, offsets)
+    device = k.device
+    _one_device(device, k_cache, k_scale, v_cache, v_scale, v, table, prefix, offsets)
     if requests == 0 or k.shape[0] == 0:
         return
-    _lib.call("v1x_kv8_store", ptr(k_cache), ptr(k_scale), ptr(v_cache), ptr(v_scale), pages, heads, ptr(k),
-              _step(k, 0), _step(k, 1), ptr(v), _step(v, 0), _step(v, 1), _DTYPES[k.dtype], k.shape[0], ptr(table),
-              _step(table, 0), table.shape[1], ptr(prefix), ptr(offsets), requests, _lib.stream_of(k),
-              device=k.device)
+    _lib.call("v1x_kv8_store", k_cache.data_ptr(), k_scale.data_ptr(), v_cache.data_ptr(), v_scale.data_ptr(), pages,
+              heads, k.data_ptr(), _step(k, 0), _step(k, 1), v.data_ptr(), _step(v, 0), _step(v, 1), code, k.shape[0],
+              table.data_ptr(), _step(table, 0), table.shape[1], prefix.data_ptr(), offsets.data_ptr(), requests,
+              _lib.stream_of(k), device=device)
 
 
 def attend(q, k_cache, k_scale, v_cache, v_scale, table, lens, scale, out=None, lse=None):
@@ -76,23 +86,26 @@ def attend(q, k_cache, k_scale, v_cache, v_scale, table, lens, scale, out=None, 
     in page ``table[r, j // 64]``.  lens int32 [rows] (at most pages * 64 count;
     negative is 0).  The tokens of a page outside the cache are no tokens."""
     pages, kv_heads = _cache(k_cache, k_scale, v_cache, v_scale)
-    require(q.dim() == 3 and q.shape[2] == 128 and q.dtype in _DTYPES, "q: [rows, heads, 128] bfloat16 or float16")
+    code = _DTYPES.get(q.dtype)
+    require(code is not None and q.dim() == 3 and q.shape[2] == 128, "q: [rows, heads, 128] bfloat16 or float16")
     rows, heads, _ = q.shape
-    require(heads >= 1 and heads % kv_heads == 0 and heads <= 1024, f"heads: a multiple of {kv_heads}, at most 1024")
+    require(1 <= heads <= 1024 and heads % kv_heads == 0, "heads: a multiple of kv_heads, at most 1024")
     require(_rows16(q), "q: unit inner stride, rows 16-byte aligned")
     require(_index(table, rows), "table: int32 [rows, pages] with unit inner stride")
-    require(lens.dtype == torch.int32 and lens.shape == (rows,) and lens.is_contiguous(),
+    require(lens.dtype is torch.int32 and lens.shape == (rows,) and lens.is_contiguous(),
             "lens: contiguous int32 [rows]")
+    scale = float(scale)
     require(math.isfinite(scale), "scale: a finite number")
     require(q.is_cuda, "q must be a CUDA tensor (there is no CPU path)")
-    _lib.same_device(q, k_cache, k_scale, v_cache, v_scale, table, lens, out, lse)
+    device = q.device
+    _one_device(device, k_cache, k_scale, v_cache, v_scale, table, lens, out, lse)
     out, lse = _outputs(q, (rows, heads, 128), out, lse)
     if rows == 0:
         return out, lse
-    size = _lib.lib().v1x_kv8_attend_workspace(rows, heads, kv_heads, table.shape[1])
-    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    _lib.call("v1x_kv8_attend", ptr(q), _step(q, 0), _step(q, 1), ptr(k_cache), ptr(k_scale), ptr(v_cache),
-              ptr(v_scale), pages, kv_heads, ptr(table), _step(table, 0), table.shape[1], ptr(lens), rows, heads,
-              float(scale), _DTYPES[q.dtype], ptr(out), ptr(lse), ptr(work), size, None, _lib.stream_of(q),
-              device=q.device)
+    size = _workspace_bytes(rows, heads, kv_heads, table.shape[1])
+    work = q.new_empty(size, dtype=torch.uint8) if size else None
+    _lib.call("v1x_kv8_attend", q.data_ptr(), _step(q, 0), _step(q, 1), k_cache.data_ptr(), k_scale.data_ptr(),
+              v_cache.data_ptr(), v_scale.data_ptr(), pages, kv_heads, table.data_ptr(), _step(table, 0),
+              table.shape[1], lens.data_ptr(), rows, heads, scale, code, out.data_ptr(), lse.data_ptr(), ptr(work), size,
+              None, _lib.stream_of(q), device=device)
     return out, lse

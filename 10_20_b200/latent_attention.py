@@ -29,6 +29,7 @@ so calls on several streams and captured graphs share nothing.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -40,57 +41,77 @@ PAGE = 64                                           # tokens per page of the nat
 _DTYPES = {torch.bfloat16: 1, torch.float16: 2}     # codes shared with v1x_pack_q
 
 
+def _rows16(t) -> bool:
+    """Unit inner stride and 16-byte aligned rows (16-bit elements)."""
+    stride = t.stride()
+    if stride[-1] == 1 and t.data_ptr() % 16 == 0:
+        for i in range(len(stride) - 1):
+            if stride[i] % 8 and t.shape[i] > 1:
+                break
+        else:
+            return True
+    return t.numel() == 0
+
+
 def _step(t, i: int) -> int:
     """The stride of dimension i; 0 where no second element is reached."""
     return t.stride(i) if t.shape[i] > 1 else 0
 
 
-def _rows16(t) -> bool:
-    """Unit inner stride and 16-byte aligned rows (16-bit elements)."""
-    return t.numel() == 0 or (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-                              and all(_step(t, i) % 8 == 0 for i in range(t.dim() - 1)))
-
-
 def _index(t, rows: int) -> bool:
     """int32 [rows, n] with unit inner stride."""
-    return t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == rows and (_step(t, 1) <= 1 or t.numel() == 0)
+    return (t.dtype is torch.int32 and t.dim() == 2 and t.shape[0] == rows
+            and (t.stride(1) == 1 or t.shape[1] <= 1 or rows == 0))
+
+
+def _one_device(device, *others) -> None:
+    for t in others:
+        require(t is None or t.device == device, "tensors on different devices")
 
 
 def _outputs(q, shape, out, lse):
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     else:
-        require(out.shape == shape and out.dtype == q.dtype and out.is_contiguous() and out.data_ptr() % 16 == 0,
-                f"out: contiguous {q.dtype} {list(shape)}, 16-byte aligned")
+        require(out.shape == shape and out.dtype is q.dtype and out.is_contiguous() and out.data_ptr() % 16 == 0,
+                "out: contiguous, of q's type, 16-byte aligned, [rows, heads, width of a value]")
     if lse is None:
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=q.device)
+        lse = q.new_empty(shape[:2], dtype=torch.float32)
     else:
-        require(lse.shape == shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous(),
-                f"lse: contiguous float32 {list(shape[:2])}")
+        require(lse.shape == shape[:2] and lse.dtype is torch.float32 and lse.is_contiguous(),
+                "lse: contiguous float32 [rows, heads]")
     return out, lse
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(rows, heads, count, latent, equal) -> int:
+    return _lib.lib().v1x_latent_attention_workspace(rows, heads, count, latent, equal)
+
+
 def _absorbed(q, pool, request_slots, index, count, lens, scale, latent, out, lse):
-    require(q.dim() == 3 and q.dtype in _DTYPES, "q: [rows, heads, dim] bfloat16 or float16")
+    code = _DTYPES.get(q.dtype)
+    require(code is not None and q.dim() == 3, "q: [rows, heads, dim] bfloat16 or float16")
     rows, heads, dim = q.shape
-    require(pool.dim() == 3 and pool.shape[1] == 1 and pool.shape[2] == dim and pool.dtype == q.dtype,
-            f"pool: [slots, 1, {dim}] of q's type")
+    require(pool.dim() == 3 and pool.shape[1] == 1 and pool.shape[2] == dim and pool.dtype is q.dtype,
+            "pool: [slots, 1, dim] of q's type, dim wide as q")
     require(latent in (128, 256, 384, 512) and dim - latent in (0, 64),
             "latent: 128, 256, 384 or 512 wide, with dim - latent 0 or 64")
     require(1 <= heads <= 1024, "heads: 1 to 1024")
     require(_rows16(q) and _rows16(pool), "q, pool: unit inner stride, rows 16-byte aligned")
+    scale = float(scale)
     require(math.isfinite(scale), "scale: a finite number")
     require(q.is_cuda, "q must be a CUDA tensor (there is no CPU path)")
-    _lib.same_device(q, pool, request_slots, index, lens, out, lse)
+    device = q.device
+    _one_device(device, pool, request_slots, index, lens, out, lse)
     out, lse = _outputs(q, (rows, heads, latent), out, lse)
     if rows == 0:
         return out, lse
-    size = _lib.lib().v1x_latent_attention_workspace(rows, heads, count, latent, lens is None)
-    work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    _lib.call("v1x_latent_attention", ptr(q), _step(q, 0), _step(q, 1), ptr(pool), pool.shape[0], _step(pool, 0),
-              ptr(request_slots), 0 if request_slots is None else request_slots.shape[0], ptr(index),
-              _step(index, 0), count, ptr(lens), rows, heads, dim, latent, float(scale), _DTYPES[q.dtype], ptr(out),
-              ptr(lse), ptr(work), size, None, _lib.stream_of(q), device=q.device)
+    size = _workspace_bytes(rows, heads, count, latent, lens is None)
+    work = q.new_empty(size, dtype=torch.uint8) if size else None
+    _lib.call("v1x_latent_attention", q.data_ptr(), _step(q, 0), _step(q, 1), pool.data_ptr(), pool.shape[0],
+              _step(pool, 0), ptr(request_slots), 0 if request_slots is None else request_slots.shape[0],
+              index.data_ptr(), _step(index, 0), count, ptr(lens), rows, heads, dim, latent, scale, code, out.data_ptr(),
+              lse.data_ptr(), ptr(work), size, None, _lib.stream_of(q), device=device)
     return out, lse
 
 
@@ -116,7 +137,7 @@ def attend_pages(q, pool, table, lens, scale, latent: int = 512, out=None, lse=N
     most pages * 64 count; negative is 0).  The tokens of a page outside the
     pool are no tokens."""
     require(_index(table, q.shape[0]), "table: int32 [rows, pages] with unit inner stride")
-    require(lens.dtype == torch.int32 and lens.shape == (q.shape[0],) and lens.is_contiguous(),
+    require(lens.dtype is torch.int32 and lens.shape == (q.shape[0],) and lens.is_contiguous(),
             "lens: contiguous int32 [rows]")
     return _absorbed(q, pool, None, table, table.shape[1] * PAGE, lens, scale, latent, out, lse)
 
@@ -133,30 +154,34 @@ def attend_prompt(q, k, k_rope, v, offsets, scale, kv_offsets=None, out=None, ls
     one projection's output or of pool rows are taken as they are.  offsets and
     kv_offsets: int32 [requests + 1], non-decreasing, within the tokens.  Rows
     of q that no request covers are left as they are in out and lse."""
-    require(q.dim() == 3 and q.dtype in _DTYPES, "q: [tokens, heads, 128 + dr] bfloat16 or float16")
+    code = _DTYPES.get(q.dtype)
+    require(code is not None and q.dim() == 3, "q: [tokens, heads, 128 + dr] bfloat16 or float16")
     tokens, heads, width = q.shape
     dr = 0 if k_rope is None else 64
-    require(width == 128 + dr, f"q: [tokens, heads, {128 + dr}]")
-    require(k.dim() == 3 and k.shape[1:] == (heads, 128) and v.shape == k.shape, f"k, v: [keys, {heads}, 128]")
+    require(width == 128 + dr, "q: [tokens, heads, 128 + dr], dr 64 with k_rope and 0 without")
     keys = k.shape[0]
-    require(k_rope is None or k_rope.shape == (keys, 64), f"k_rope: [{keys}, 64]")
-    require(all(t.dtype == q.dtype and _rows16(t) for t in (q, k, v, k_rope) if t is not None),
+    require(k.shape == (keys, heads, 128) and v.shape == k.shape, "k, v: [keys, heads, 128], heads as in q")
+    require(k_rope is None or k_rope.shape == (keys, 64), "k_rope: [keys, 64]")
+    require(k.dtype is q.dtype and v.dtype is q.dtype and (k_rope is None or k_rope.dtype is q.dtype)
+            and _rows16(q) and _rows16(k) and _rows16(v) and (k_rope is None or _rows16(k_rope)),
             "q, k, k_rope, v: one type, unit inner stride, rows 16-byte aligned")
     require(1 <= heads <= 1024, "heads: 1 to 1024")
+    scale = float(scale)
     require(math.isfinite(scale), "scale: a finite number")
     if kv_offsets is None:
         kv_offsets = offsets
-    require(all(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() for t in (offsets, kv_offsets))
-            and offsets.shape == kv_offsets.shape and offsets.shape[0] >= 1,
-            "offsets, kv_offsets: contiguous int32 [requests + 1]")
+    require(offsets.dtype is torch.int32 and kv_offsets.dtype is torch.int32 and offsets.dim() == 1
+            and offsets.is_contiguous() and kv_offsets.is_contiguous() and offsets.shape == kv_offsets.shape
+            and offsets.shape[0] >= 1, "offsets, kv_offsets: contiguous int32 [requests + 1]")
     require(q.is_cuda, "q must be a CUDA tensor (there is no CPU path)")
-    _lib.same_device(q, k, k_rope, v, offsets, kv_offsets, out, lse)
+    device = q.device
+    _one_device(device, k, k_rope, v, offsets, kv_offsets, out, lse)
     out, lse = _outputs(q, (tokens, heads, 128), out, lse)
     requests = offsets.shape[0] - 1
     if tokens == 0 or requests == 0:
         return out, lse
-    _lib.call("v1x_prompt_attention", ptr(q), _step(q, 0), _step(q, 1), ptr(k), _step(k, 0), _step(k, 1), ptr(k_rope),
-              0 if k_rope is None else _step(k_rope, 0), ptr(v), _step(v, 0), _step(v, 1), ptr(offsets),
-              ptr(kv_offsets), requests, tokens, keys, heads, dr, float(scale), _DTYPES[q.dtype], ptr(out), ptr(lse),
-              None, _lib.stream_of(q), device=q.device)
+    _lib.call("v1x_prompt_attention", q.data_ptr(), _step(q, 0), _step(q, 1), k.data_ptr(), _step(k, 0), _step(k, 1),
+              ptr(k_rope), 0 if k_rope is None else _step(k_rope, 0), v.data_ptr(), _step(v, 0), _step(v, 1),
+              offsets.data_ptr(), kv_offsets.data_ptr(), requests, tokens, keys, heads, dr, scale, code, out.data_ptr(),
+              lse.data_ptr(), None, _lib.stream_of(q), device=device)
     return out, lse
