@@ -2,9 +2,9 @@
 // in v1x.h.
 //
 // A CTA has 256 queries of one request and head, two tiles of 128, and goes over
-// the keys that they see in tiles of 128:
+// the keys that they see:
 //
-//   S_t[128 x 128]  = Q_t . [K | K_rope]^T    K = 128 + dr, operands in shared memory
+//   S_t[128 x 64]   = Q_t . [K | K_rope]^T    K = 128 + dr, operands in shared memory
 //   O_t[128 x 128] += P_t . V                 P in TMEM, over S_t
 //
 // One query per TMEM lane: a softmax thread owns a query's row, so maxima, sums and
@@ -13,19 +13,26 @@
 // a few times a row at most; sums stay in 32 bits, the weights are rounded once, to
 // the inputs' type, for the second product.
 //
-// The tensor cores alternate between the tiles (S_0, O_1, S_1, O_0, ...), so that one
-// tile's softmax runs beside the other's products: 2560 cycles of MMA per 128 keys
-// with dr = 64 against 2048 of exp2 for both tiles, at the hardware's rates.
+// Keys go in steps of 64, two score buffers a tile: while a tile's softmax is at one
+// step, the tensor cores form the output of the step before and, once that has read
+// its weights, the scores of the step after over them.  Per 128 keys with dr = 64 the
+// tensor cores need 3328 cycles (a 128 x 64 x 16 MMA takes 48, bound by shared
+// memory; 128-key steps would need 2560, but with one buffer a tile the chain S,
+// softmax, O, S took 4900), the special-function units 2048.
 // 96 KB of queries leave room for three 32 KB slots that keys and values take in
-// turn and two 16 KB slots of rotary keys; the rows come by 16-byte cp.async, which
-// takes any strides and writes zeros past the request's last key (a neighbour's
-// values never enter a product).
+// turn and two 16 KB slots of rotary keys.  Whole tiles come by TMA (a slot that is
+// free is full 1100 cycles later; by cp.async, whose 48 instructions a warp took 1500
+// to issue, it was 3200, more than the ring hides); a request's last tile, and tensors
+// whose heads share memory, come by 16-byte cp.async, which writes zeros past the last
+// key (a neighbour's values never enter a product) and takes any strides.
 //
 // Warp roles (384 threads, one CTA per SM): 0-3 and 4-7 softmax and epilogue of the
-// two tiles, 8 TMEM owner and MMA issuer, 9-10 keys and values (64 rows each), 11
-// the queries, then the rotary keys.  Later queries see more keys: the grid begins
-// with the last ones, all heads of a tile side by side.
+// two tiles, 8 and 9 issue their MMAs (8 owns the TMEM), 10 and 11 bring the queries,
+// then keys and values.  Later queries see more keys: the grid begins with the last
+// ones, all heads of a tile side by side.
 // Waits are bounded (2 s, then V1X_STATUS_TIMEOUT).
+#include <cudaTypedefs.h>
+
 #include <type_traits>
 
 #include "attention.cuh"
@@ -38,6 +45,7 @@ using namespace attn;
 using namespace sm100;
 
 constexpr int kRows = 128;                // queries of a tile, keys of a tile
+constexpr int kStep = 64;                 // keys of a step: half of a key tile
 constexpr int kBlock = kRows * 128;       // bytes of 64 elements of a tile's rows
 constexpr int kThreads = 384;
 constexpr int kSlots = 3, kRopeSlots = 2;
@@ -55,11 +63,12 @@ struct PromptArgs {
   void* out;
   float* lse;
   int32_t* status;
+  int tma;               // the tensor maps are there
 };
 
 struct PromptShared {
-  uint64_t full[kSlots], empty[kSlots], rope_full[kRopeSlots], rope_empty[kRopeSlots];
-  uint64_t q_full, s_full[2], p_full[2], pv_done[2], o_done;
+  uint64_t full[kSlots], empty[kSlots], rope_empty[kRopeSlots];   // keys: with their rotary part
+  uint64_t q_full, s_full[2][2], p_full[2][2], pv_done[2][2], o_done[2];   // [tile][step & 1]
   int64_t request;
   uint32_t tmem;
   int abort, zero;
@@ -102,7 +111,9 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, int R0, const char* src,
 }
 
 template <typename T, bool kRope>
-__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs a) {
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                  const __grid_constant__ CUtensorMap rope_map, const __grid_constant__ PromptArgs a) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kQBlocks = kRope ? 3 : 2;
   extern __shared__ uint8_t smem_raw[];
@@ -132,33 +143,32 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
   const int64_t nq = q1 - q0, nk = k1 - k0, tile = unit - (q0 / 256 + r);
   const int64_t i0 = tile * 256;                           // the first query of the request in this CTA
   if (tile < 0 || i0 >= nq) return;
-  // key tiles that a tile of queries sees: up to its last query's limit
-  auto tiles_seen = [&](int t) {
+  // steps of 64 keys that a tile of queries sees: up to its last query's limit
+  auto steps_seen = [&](int t) {
     const int64_t last = min(i0 + 128 * (t + 1), nq) - 1;
     if (last < i0 + 128 * t) return 0;
     const int64_t limit = min(last + 1 + nk - nq, nk);
-    return limit > 0 ? static_cast<int>((limit + kRows - 1) / kRows) : 0;
+    return limit > 0 ? static_cast<int>((limit + kStep - 1) / kStep) : 0;
   };
-  const int n0 = tiles_seen(0), n1 = tiles_seen(1), n = max(n0, n1);
+  const int n0 = steps_seen(0), n1 = steps_seen(1), n = (max(n0, n1) + 1) / 2;   // n: key tiles
 
   if (tid == 0) {
     sh.abort = 0;
     sh.zero = 0;
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&sh.full[i], 2);
-      mbar_init(&sh.empty[i], 1);
+      mbar_init(&sh.empty[i], 2);
     }
-    for (int i = 0; i < kRopeSlots; ++i) {
-      mbar_init(&sh.rope_full[i], 1);
-      mbar_init(&sh.rope_empty[i], 1);
-    }
+    for (int i = 0; i < kRopeSlots; ++i) mbar_init(&sh.rope_empty[i], 2);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
-      mbar_init(&sh.pv_done[i], 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&sh.s_full[i][x], 1);
+        mbar_init(&sh.p_full[i][x], 4);
+        mbar_init(&sh.pv_done[i][x], 1);
+      }
+      mbar_init(&sh.o_done[i], 1);
     }
-    mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.o_done, 1);
+    mbar_init(&sh.q_full, 2);
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -181,22 +191,26 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const float c = a.scale_log2;
     float m = -CUDART_INF_F, l = 0.0f;       // m: of the unscaled scores
     bool ok = true;
-    for (int j = 0; j < mine; ++j) {
-      if (ok && !mbar_wait(&sh.s_full[t], j & 1, &sh.abort, kWaitNs)) {
+    auto wait = [&](uint64_t* bar, int phase) {
+      if (ok && !mbar_wait(bar, phase & 1, &sh.abort, kWaitNs)) {
         give_up(sh, a.status);
         ok = false;
       }
+    };
+    for (int j = 0; j < mine; ++j) {
+      const int x = j & 1;
+      wait(&sh.s_full[t][x], j >> 1);
       if (__any_sync(0xffffffffu, !ok)) break;
       tc_fence_after();
-      uint32_t s[4][32];
+      uint32_t s[2][32];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) tmem_ld32(s_addr + 32 * b, s[b]);
+      for (int b = 0; b < 2; ++b) tmem_ld32(s_addr + kStep * x + 32 * b, s[b]);
       tmem_ld_wait();
-      if (__any_sync(0xffffffffu, limit < static_cast<int64_t>(j + 1) * kRows)) {
-        const int left = static_cast<int>(max(min(limit - static_cast<int64_t>(j) * kRows, static_cast<int64_t>(kRows)),
+      if (__any_sync(0xffffffffu, limit < static_cast<int64_t>(j + 1) * kStep)) {
+        const int left = static_cast<int>(max(min(limit - static_cast<int64_t>(j) * kStep, static_cast<int64_t>(kStep)),
                                               static_cast<int64_t>(0)));
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (32 * b + e >= left) s[b][e] = 0xFF800000u;   // -inf
@@ -204,20 +218,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       float top[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        top[b] = __uint_as_float(s[b][0]);
+        top[b] = __uint_as_float(s[b >> 1][16 * (b & 1)]);
 #pragma unroll
-        for (int e = 1; e < 32; ++e) top[b] = fmaxf(top[b], __uint_as_float(s[b][e]));
+        for (int e = 1; e < 16; ++e) top[b] = fmaxf(top[b], __uint_as_float(s[b >> 1][16 * (b & 1) + e]));
       }
       const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
       if (j == 0) {
         m = most;
       } else {
-        // s_full says that every product issued before is complete, O's included
         const bool grows = m == -CUDART_INF_F ? most > m : (most - m) * c > kLazy;
         if (__any_sync(0xffffffffu, grows)) {
           const float f = grows ? (m == -CUDART_INF_F ? 0.0f : exp2_fast((m - most) * c)) : 1.0f;
           if (grows) m = most;
           l *= f;
+          wait(&sh.pv_done[t][x ^ 1], (j - 1) >> 1);   // O holds all that was given to it
+          __syncwarp();
+          tc_fence_after();
 #pragma unroll 1
           for (int b = 0; b < 4; ++b) {
             uint32_t o[32];
@@ -231,25 +247,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       }
       const float shift = m == -CUDART_INF_F ? 0.0f : -m * c;
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      uint32_t w[32];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[32];
-#pragma unroll
-        for (int e = 0; e < 64; e += 2) {
-          const float u = exp2_fast(fmaf(__uint_as_float(s[2 * half + (e >> 5)][e & 31]), c, shift));
-          const float v = exp2_fast(fmaf(__uint_as_float(s[2 * half + (e >> 5)][(e & 31) + 1]), c, shift));
-          sum[(e >> 1) & 3] += u + v;
-          w[e >> 1] = pack2<T>(u, v);
-        }
-        tmem_st32(s_addr + 32 * half, w);
+      for (int e = 0; e < 64; e += 2) {
+        const float u = exp2_fast(fmaf(__uint_as_float(s[e >> 5][e & 31]), c, shift));
+        const float v = exp2_fast(fmaf(__uint_as_float(s[e >> 5][(e & 31) + 1]), c, shift));
+        sum[(e >> 1) & 3] += u + v;
+        w[e >> 1] = pack2<T>(u, v);
       }
+      tmem_st32(s_addr + kStep * x, w);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full[t]);
+      if (lane == 0) mbar_arrive(&sh.p_full[t][x]);
     }
-    if (mine > 0 && ok && !mbar_wait(&sh.o_done, 0, &sh.abort, kWaitNs)) give_up(sh, a.status);
+    if (mine > 0 && ok && !mbar_wait(&sh.o_done[t], 0, &sh.abort, kWaitNs)) give_up(sh, a.status);
     __syncwarp();
     tc_fence_after();
     const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
@@ -276,122 +289,139 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     if (i < nq)
       a.lse[(q0 + i) * a.heads + h] = l > 0.0f ? (m * c + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
     tc_fence_before();
-  } else if (warp == 8) {
-    // ---------------- MMA issuer ----------------
-    if (n > 0) {
-      const uint32_t qk = idesc_16bit_f32(kBf16, 128, 128, false, false) | (a.negative ? 1u << 13 : 0u);
-      const uint32_t pv = idesc_16bit_f32(kBf16, 128, 128, false, true);
-      bool ok = converged_wait(sh, a.status, &sh.q_full, 0);
-      int issued = 0;
-      auto scores = [&](int t, int j) {
-        const int u = 2 * j, slot = u % kSlots, rope = j % kRopeSlots;
-        const bool last = t == 1 || j >= n1;
-        ok = ok && converged_wait(sh, a.status, &sh.full[slot], u / kSlots);
-        if (kRope) ok = ok && converged_wait(sh, a.status, &sh.rope_full[rope], j / kRopeSlots);
-        if (j > 0) ok = ok && converged_wait(sh, a.status, &sh.pv_done[t], j - 1);   // P_t is read: S_t may be written
-        if (!ok) return;
-        const uint32_t qd = desc_k(q_smem + t * kQBlocks * kBlock), kd = desc_k(kv_smem + slot * 2 * kBlock);
-        const uint32_t rd = desc_k(rope_smem + rope * kBlock), d = tmem + 128 * t;
+  } else if (warp < 10) {
+    // ---------------- MMA issuers, one per tile ----------------
+    const int t = warp - 8, mine = t ? n1 : n0;
+    const uint32_t qk = idesc_16bit_f32(kBf16, 128, kStep, false, false) | (a.negative ? 1u << 13 : 0u);
+    const uint32_t pv = idesc_16bit_f32(kBf16, 128, 128, false, true);
+    const uint32_t s_tmem = tmem + 128 * t, o_tmem = tmem + kOutCol + 128 * t;
+    const uint32_t qd = desc_k(q_smem + t * kQBlocks * kBlock);
+    bool ok = true, issued = false;
+    auto wait = [&](uint64_t* bar, int phase) { return ok = ok && converged_wait(sh, a.status, bar, phase); };
+    // key tile j in slot 2 j of the ring (mod kSlots), its values in slot 2 j + 1
+    auto scores = [&](int j) {                   // of step j
+      const int u = j & ~1, slot = u % kSlots, rope = (j >> 1) % kRopeSlots, x = j & 1;
+      if (x == 0) wait(&sh.full[slot], u / kSlots);
+      if (j >= 2) wait(&sh.pv_done[t][x], (j - 2) >> 1);   // the weights are read: S may be written over them
+      if (!ok) return;
+      const uint32_t kd = desc_k(kv_smem + slot * 2 * kBlock + x * (kBlock / 2));
+      const uint32_t rd = desc_k(rope_smem + rope * kBlock + x * (kBlock / 2)), d = s_tmem + kStep * x;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16(d, qd + (b * kBlock + 32 * k) / 16, kd + (b * kBlock + 32 * k) / 16, qk, b + k > 0 ? 1u : 0u);
-        if (kRope) {
+        for (int k = 0; k < 4; ++k)
+          umma_f16(d, qd + (b * kBlock + 32 * k) / 16, kd + (b * kBlock + 32 * k) / 16, qk, b + k > 0 ? 1u : 0u);
+      if (kRope) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(d, qd + (2 * kBlock + 32 * k) / 16, rd + 32 * k / 16, qk, 1u);
-        }
-        umma_commit_elect(&sh.s_full[t]);
-        if (last) {
-          umma_commit_elect(&sh.empty[slot]);
-          if (kRope) umma_commit_elect(&sh.rope_empty[rope]);
-        }
-        issued = 1;
-      };
-      auto output = [&](int t, int j) {
-        const int u = 2 * j + 1, slot = u % kSlots;
-        const bool last = t == 1 || j >= n1;
-        ok = ok && converged_wait(sh, a.status, &sh.full[slot], u / kSlots);
-        ok = ok && converged_wait(sh, a.status, &sh.p_full[t], j);
-        if (!ok) return;
-        const uint32_t vd = desc_mn(kv_smem + slot * 2 * kBlock, kBlock), d = tmem + kOutCol + 128 * t, p = tmem + 128 * t;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) umma_f16_ta(d, p + 8 * k, vd + 2048 * k / 16, pv, j + k > 0 ? 1u : 0u);
-        umma_commit_elect(&sh.pv_done[t]);
-        if (last) umma_commit_elect(&sh.empty[slot]);
-      };
-      if (n0 > 0) scores(0, 0);
-      if (n1 > 0) scores(1, 0);
-      for (int j = 0; j < n && ok; ++j) {
-        if (j < n0) {
-          output(0, j);
-          if (j + 1 < n0) scores(0, j + 1);
-        }
-        if (j < n1) {
-          output(1, j);
-          if (j + 1 < n1) scores(1, j + 1);
-        }
+        for (int k = 0; k < 4; ++k) umma_f16(d, qd + (2 * kBlock + 32 * k) / 16, rd + 32 * k / 16, qk, 1u);
       }
-      // everything that was issued retires before the CTA ends
-      if (issued) {
-        umma_commit_elect(&sh.o_done);
-        mbar_wait(&sh.o_done, 0, &sh.zero, kWaitNs);
+      umma_commit_elect(&sh.s_full[t][x]);
+      if (x == 1 || j == mine - 1) {
+        umma_commit_elect(&sh.empty[slot]);
+        if (kRope) umma_commit_elect(&sh.rope_empty[rope]);
       }
+      issued = true;
+    };
+    auto output = [&](int j) {
+      const int u = j | 1, slot = u % kSlots, x = j & 1;
+      if (x == 0) wait(&sh.full[slot], u / kSlots);
+      wait(&sh.p_full[t][x], j >> 1);
+      if (!ok) return;
+      const uint32_t vd = desc_mn(kv_smem + slot * 2 * kBlock + x * (kBlock / 2), kBlock), p = s_tmem + kStep * x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) umma_f16_ta(o_tmem, p + 8 * k, vd + 2048 * k / 16, pv, j + k > 0 ? 1u : 0u);
+      umma_commit_elect(&sh.pv_done[t][x]);
+      if (x == 1 || j == mine - 1) umma_commit_elect(&sh.empty[slot]);
+    };
+    if (mine > 0) wait(&sh.q_full, 0);
+    if (mine > 0 && ok) scores(0);
+    if (mine > 1 && ok) scores(1);
+    for (int j = 0; j < mine && ok; ++j) {
+      output(j);
+      if (j + 2 < mine && ok) scores(j + 2);
     }
-  } else if (warp < 11) {
-    // ---------------- keys and values ----------------
-    const int half = warp - 9;
+    for (int u = 2 * ((mine + 1) / 2); u < 2 * n && ok; ++u) {   // the other tile's alone
+      wait(&sh.full[u % kSlots], u / kSlots);
+      if (lane == 0) {
+        mbar_arrive(&sh.empty[u % kSlots]);
+        if (kRope && !(u & 1)) mbar_arrive(&sh.rope_empty[(u >> 1) % kRopeSlots]);
+      }
+      __syncwarp();
+    }
+    // everything that was issued retires before the CTA ends
+    if (issued) {
+      umma_commit_elect(&sh.o_done[t]);
+      mbar_wait(&sh.o_done[t], 0, &sh.zero, kWaitNs);
+    }
+  } else if (n > 0) {
+    // ---------------- queries, keys, values: 64 rows of a tile per warp ----------------
+    const int half = warp - 10;
+    const char* const q = static_cast<const char*>(a.q) + (q0 * a.qs0 + h * a.qs1) * 2;
     const char* const k = static_cast<const char*>(a.k) + (k0 * a.ks0 + h * a.ks1) * 2;
     const char* const v = static_cast<const char*>(a.v) + (k0 * a.vs0 + h * a.vs1) * 2;
-    int pending = -1;                            // a load whose arrival has not been reported
+    const char* const kr = static_cast<const char*>(a.k_rope) + k0 * a.krs0 * 2;
+    for (int t = 0; t < 2; ++t)
+      copy_tile<kQBlocks, 64>(q_smem + t * kQBlocks * kBlock, 64 * half, q, a.qs0 * 2, i0 + 128 * t + 64 * half, nq, a.q, lane);
+    cp_async_commit();
+    uint64_t* pending = &sh.q_full;              // a load whose arrival has not been reported
     auto report = [&] {
       fence_async_shared();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.full[pending % kSlots]);
+      if (lane == 0) mbar_arrive(pending);
     };
+    int slot = 0, turn = 0;
     for (int u = 0; u < 2 * n; ++u) {
-      const int slot = u % kSlots, phase = ((u / kSlots) & 1) ^ 1;
-      if (pending >= 0 && !__all_sync(0xffffffffu, mbar_test(&sh.empty[slot], phase))) {
+      const int j = u >> 1, rope = j % kRopeSlots;
+      const bool keys = (u & 1) == 0;
+      if (pending && !__all_sync(0xffffffffu, mbar_test(&sh.empty[slot], (turn & 1) ^ 1))) {
         cp_async_wait<0>();
         report();
-        pending = -1;
+        pending = nullptr;
       }
-      if (!converged_wait(sh, a.status, &sh.empty[slot], phase)) break;
-      const int64_t row = static_cast<int64_t>(u >> 1) * kRows + 64 * half;
-      copy_tile<2, 64>(kv_smem + slot * 2 * kBlock, 64 * half, u & 1 ? v : k, (u & 1 ? a.vs0 : a.ks0) * 2, row, nk, a.q, lane);
+      if (!converged_wait(sh, a.status, &sh.empty[slot], turn ^ 1)) break;
+      if (kRope && keys && !converged_wait(sh, a.status, &sh.rope_empty[rope], (j / kRopeSlots) ^ 1)) break;
+      if (a.tma && static_cast<int64_t>(j + 1) * kRows <= nk) {   // whole tiles come by TMA
+        if (pending) {
+          cp_async_wait<0>();
+          report();
+          pending = nullptr;
+        }
+        if (lane == 0) {
+          uint64_t* const bar = &sh.full[slot];
+          uint8_t* const to = base + (6 + slot * 2) * kBlock;
+          const int y = static_cast<int>(h), z = static_cast<int>(k0) + j * kRows;
+          if (half == 1) {
+            mbar_arrive(bar);
+          } else {
+            mbar_arrive_expect_tx(bar, kRope && keys ? 3 * kBlock : 2 * kBlock);
+            tma_load_3d(to, keys ? &k_map : &v_map, bar, 0, y, z);
+            tma_load_3d(to + kBlock, keys ? &k_map : &v_map, bar, 64, y, z);
+            if (kRope && keys) tma_load_2d(base + (6 + 2 * kSlots + rope) * kBlock, &rope_map, bar, 0, z);
+          }
+        }
+        __syncwarp();
+        if (++slot == kSlots) {
+          slot = 0;
+          ++turn;
+        }
+        continue;
+      }
+      const int64_t row = static_cast<int64_t>(j) * kRows + 64 * half;
+      copy_tile<2, 64>(kv_smem + slot * 2 * kBlock, 64 * half, keys ? k : v, (keys ? a.ks0 : a.vs0) * 2, row, nk, a.q, lane);
+      if (kRope && keys) copy_tile<1, 64>(rope_smem + rope * kBlock, 64 * half, kr, a.krs0 * 2, row, nk, a.q, lane);
       cp_async_commit();
-      if (pending >= 0) {
+      if (pending) {
         cp_async_wait<1>();
         report();
       }
-      pending = u;
-    }
-    cp_async_wait_all();
-    if (pending >= 0) report();
-  } else {
-    // ---------------- queries, rotary keys ----------------
-    if (n > 0) {
-      const char* const q = static_cast<const char*>(a.q) + (q0 * a.qs0 + h * a.qs1) * 2;
-      for (int t = 0; t < 2; ++t)
-        copy_tile<kQBlocks, 128>(q_smem + t * kQBlocks * kBlock, 0, q, a.qs0 * 2, i0 + 128 * t, nq, a.q, lane);
-      cp_async_wait_all();
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.q_full);
-      if (kRope) {
-        const char* const kr = static_cast<const char*>(a.k_rope) + k0 * a.krs0 * 2;
-        for (int j = 0; j < n; ++j) {
-          const int slot = j % kRopeSlots;
-          if (!converged_wait(sh, a.status, &sh.rope_empty[slot], (j / kRopeSlots) ^ 1)) break;
-          copy_tile<1, 128>(rope_smem + slot * kBlock, 0, kr, a.krs0 * 2, static_cast<int64_t>(j) * kRows, nk, a.q, lane);
-          cp_async_wait_all();
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.rope_full[slot]);
-        }
-        cp_async_wait_all();
+      pending = &sh.full[slot];
+      if (++slot == kSlots) {
+        slot = 0;
+        ++turn;
       }
     }
+    cp_async_wait_all();
+    if (pending) report();
   }
   __syncthreads();
   if (warp == 8) {
@@ -403,13 +433,56 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 constexpr int kSmem = 1024 + (6 + 2 * kSlots + kRopeSlots) * kBlock + static_cast<int>(sizeof(PromptShared));
 static_assert(kSmem <= 232448, "shared memory");
 
+// Rows [keys][heads] of 128 elements as boxes of 64 elements x 128 keys of one head
+// (heads = 0: rows [keys] of 64 elements), 128-byte swizzle.  False where the driver
+// takes no such map.
+bool encode_rows(CUtensorMap* map, bool bf16, const void* p, int64_t keys, int64_t heads, int64_t key_stride,
+                 int64_t head_stride) {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  if (!fn) return false;
+  const cuuint32_t steps[3] = {1, 1, 1};
+  const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r;
+  if (heads) {
+    const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(keys)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride * 2), static_cast<cuuint64_t>(key_stride * 2)};
+    const cuuint32_t box[3] = {64, 1, kRows};
+    r = fn(map, type, 3, const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  } else {
+    const cuuint64_t dims[2] = {64, static_cast<cuuint64_t>(keys)}, strides[1] = {static_cast<cuuint64_t>(key_stride * 2)};
+    const cuuint32_t box[2] = {64, kRows};
+    r = fn(map, type, 2, const_cast<void*>(p), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
+  return r == CUDA_SUCCESS;
+}
+
 template <typename T, bool kRope>
-void launch(const PromptArgs& a, cudaStream_t s) {
+void launch(PromptArgs a, cudaStream_t s) {
+  // Maps for the whole tiles.  Strides of 0 (a dimension of one, or a broadcast one)
+  // take no map: a dimension of one gets any stride, broadcast tensors go without.
+  CUtensorMap k_map = {}, v_map = {}, rope_map = {};
+  auto stride = [](int64_t given, int64_t count) { return given == 0 && count == 1 ? int64_t(128) : given; };
+  const int64_t ks0 = stride(a.ks0, a.keys), ks1 = stride(a.ks1, a.heads), vs0 = stride(a.vs0, a.keys), vs1 = stride(a.vs1, a.heads);
+  const int64_t krs0 = stride(a.krs0, a.keys);
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  a.tma = a.keys >= kRows && ks0 > 0 && ks1 > 0 && vs0 > 0 && vs1 > 0 && (!kRope || krs0 > 0) &&
+          encode_rows(&k_map, kBf16, a.k, a.keys, a.heads, ks0, ks1) &&
+          encode_rows(&v_map, kBf16, a.v, a.keys, a.heads, vs0, vs1) &&
+          (!kRope || encode_rows(&rope_map, kBf16, a.k_rope, a.keys, 0, krs0, 0));
   static DeviceOnce once;
   once.run([] { cudaFuncSetAttribute(prompt_kernel<T, kRope>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem); });
   launch_kernel_prio(LaunchPriority::kDefault, prompt_kernel<T, kRope>,
                      dim3(static_cast<unsigned>(a.heads), static_cast<unsigned>(a.tokens / 256 + a.requests)),
-                     dim3(kThreads), kSmem, s, a);
+                     dim3(kThreads), kSmem, s, k_map, v_map, rope_map, a);
 }
 
 }  // namespace
@@ -438,7 +511,7 @@ extern "C" int v1x_prompt_attention(const void* q, int64_t qs0, int64_t qs1, con
   // a masked score, -inf, has to stay -inf under the scale
   const float magnitude = scale == 0 ? 1e-30f : (scale < 0 ? -scale : scale) * kLog2e;
   const PromptArgs a{q,    k,     k_rope, v, qs0, qs1, ks0, ks1, krs0, vs0, vs1, offsets, kv_offsets, requests, tokens,
-                     keys, heads, magnitude, scale < 0 ? 1 : 0, out, lse, status};
+                     keys, heads, magnitude, scale < 0 ? 1 : 0, out, lse, status, 0};
   cudaStream_t s = as_stream(stream);
   if (dtype == 1) dr ? launch<__nv_bfloat16, true>(a, s) : launch<__nv_bfloat16, false>(a, s);
   else dr ? launch<__half, true>(a, s) : launch<__half, false>(a, s);

@@ -271,6 +271,18 @@ def test_prompt_poison_and_uncovered_rows():
     assert (out[keep] == 5).all() and (lse[keep] == 5).all()
 
 
+def test_prompt_shared_heads_and_strides():
+    """Keys and values broadcast over the heads (stride 0), and heads outside the tokens, equal to their copies."""
+    q, kv, kr = normal((300, 3, 192), "bf16", 44), normal((300, 1, 256), "bf16", 45), normal((300, 64), "bf16", 46)
+    k, v = kv[..., :128].expand(300, 3, 128), kv[..., 128:].expand(300, 3, 128)
+    off = ints([0, 300])
+    a = L.attend_prompt(q, k, kr, v, off, 0.08)
+    check(*a, want_prompt(q, k, kr, v, [0, 300], [0, 300], 0.08, "bf16"))
+    swapped = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    b = L.attend_prompt(swapped[0], swapped[1], kr, swapped[2], off, 0.08)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_prompt_neighbours_do_not_leak():
     """A request's result does not depend on what its neighbours in the same tiles hold."""
     q, kv, kr = normal((300, 2, 192), "fp16", 36), normal((300, 2, 256), "fp16", 37), normal((300, 64), "fp16", 38)
