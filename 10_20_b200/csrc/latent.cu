@@ -144,8 +144,11 @@ __device__ __forceinline__ void give_up(LatentShared& sh, int32_t* status) {
 
 // A whole warp waits, and agrees on the outcome.
 __device__ __forceinline__ bool converged_wait(LatentShared& sh, int32_t* status, uint64_t* bar, int phase) {
-  const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, &sh.abort, kWaitNs));
-  if (!ok) give_up(sh, status);
+  bool ok = __all_sync(0xffffffffu, mbar_test(bar, phase & 1));   // most phases are complete when asked for
+  if (!ok) {
+    ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, &sh.abort, kWaitNs));
+    if (!ok) give_up(sh, status);
+  }
   tc_fence_after();
   return ok;
 }
