@@ -28,17 +28,17 @@
 // in the workspace, joined by latent_join_kernel in the order of the ranges; rows
 // of equal length are given to the CTAs whole where that is no longer (cut_for).
 //
-// Warp roles (480 threads, one CTA per SM):
+// Warp roles (512 threads, one CTA per SM):
 //   0-3   softmax, rescale, epilogue (TMEM lane quarters 0-3)
 //   4-11  four sets of two producer warps, a half of every other tile each: rows by
 //         16-byte cp.async into the swizzled layout, each row's slot looked up a
 //         tile ahead; a token that is none becomes zeros and a cleared bit of the
 //         tile's mask
-//   12    TMEM owner; issues the scores' MMAs, up to two tiles ahead
-//   13    issues the outputs' MMAs: an MMA of these shapes takes 32 to 48 cycles and
-//         few are queued, so one warp's waits between the two products left the
-//         tensor cores idle (111 us instead of 92 on the decode batch)
-//   14    the queries, when the row changes
+//   12, 14  issue the scores' MMAs of even and odd tiles (12 owns the TMEM); 13 the
+//         outputs', a half of a tile at a time.  An MMA of these shapes takes 32 to 48
+//         cycles and few are queued: one warp's waits between the two products left
+//         the tensor cores idle (111 us instead of 92 on the decode batch)
+//   15    the queries, when the row changes
 // Waits are bounded (2 s, then V1X_STATUS_TIMEOUT).
 #include <type_traits>
 
@@ -55,7 +55,7 @@ constexpr int kTile = 64;                // tokens of a tile, in two halves
 constexpr int kGroup = 64;               // heads of a CTA
 constexpr int kBlock = 64 * 128;         // bytes of 64 elements of 64 rows (queries, tokens) or of the weights
 constexpr int kMaxPairs = 4;             // tiles in shared memory: 2, or 4 where they fit
-constexpr int kThreads = 480;
+constexpr int kThreads = 512;
 constexpr int kMaxCtas = 148;
 constexpr uint32_t kScoreCol = 256;      // TMEM: O^T in columns 0-255, two score tiles after it
 constexpr float kLazy = 8.0f;            // log2 of the growth that the weights may show before a rescale
@@ -84,12 +84,16 @@ struct LatentArgs {
   int32_t* status;
 };
 
+// what a tile is in its segment (the tiles of one row in a CTA's range; segments
+// are counted from kSegment on)
+constexpr uint32_t kFirst = 1, kLastOfRow = 2, kBeforeLast = 4, kSegment = 8;
+
 struct LatentShared {
   uint64_t full[2 * kMaxPairs];    // of a tile: its first blocks, all of it
   uint64_t empty[2 * kMaxPairs];   // its halves
-  uint64_t s_full[2], p_full[2], pv_done, q_full, q_empty;
+  uint64_t s_full[2], p_full[2][2], pv_done[2], q_full, q_empty;   // p_full, pv_done: of a tile's halves
   uint64_t mask[kMaxPairs];
-  uint32_t flags[kMaxPairs];   // 1: the first tile of a segment, 2: the last of a row
+  uint32_t flags[kMaxPairs];
   alignas(16) float factor[kGroup];
   int64_t start[4];  // as LatentArgs::where, but [3]: all tiles
   int64_t cut[2];    // base, extra
@@ -219,11 +223,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.p_full[i][0], 4);
+      mbar_init(&sh.p_full[i][1], 4);
+      mbar_init(&sh.pv_done[i], 1);
     }
-    mbar_init(&sh.pv_done, 1);
     mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.q_empty, 2);
     fence_mbar_init();
   }
   if (warp == 12) {
@@ -299,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     // four warps still meet at their barriers
     bool ok = true;
     auto wait = [&](uint64_t* bar, int phase) {
-      if (ok && !mbar_wait(bar, phase & 1, &sh.abort, kWaitNs)) {
+      if (ok && !mbar_test(bar, phase & 1) && !mbar_wait(bar, phase & 1, &sh.abort, kWaitNs)) {
         give_up(sh, a.status);
         ok = false;
       }
@@ -341,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
           if (grows) m = most;
           l *= f;
           if (mine) sh.factor[h] = f;
-          wait(&sh.pv_done, it - 1);
+          wait(&sh.pv_done[1], it - 1);
           sync_128();
           tc_fence_after();
           for (int t = 0; t < kOut; ++t)
@@ -360,33 +365,38 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       fresh = false;
       const float ref = m == -CUDART_INF_F ? 0.0f : m;
       float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      // the halves' weights are handed over one after the other
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        s[j] = exp2_fast(s[j] - ref);
-        sum[j & 3] += s[j];
+      for (int half = 0; half < 2; ++half) {
+        float* const e = s + 16 * half;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          e[j] = exp2_fast(e[j] - ref);
+          sum[j & 3] += e[j];
+        }
+        // neighbouring tokens' weights meet in one thread: the half's tokens 0-15 in the
+        // even one, 16-31 in the odd one
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float got = __shfl_xor_sync(0xffffffffu, odd ? e[j] : e[j + 8], 2);
+          w[j] = odd ? pack2<T>(got, e[j + 8]) : pack2<T>(e[j], got);
+        }
+        // their buffer is free once the previous tile's product has read it
+        if (it > 0) wait(&sh.pv_done[half], it - 1);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<uint4*>(p_ptr + h * 128 + (((half * 4 + odd * 2 + c) ^ (h & 7)) << 4)) =
+              make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        fence_async_shared();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[it & 1][half]);
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      // neighbouring tokens' weights meet in one thread: tokens 0-31 of the tile in
-      // the even one, 32-63 in the odd one
-      uint32_t w[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float got = __shfl_xor_sync(0xffffffffu, odd ? s[j] : s[j + 16], 2);
-        w[j] = odd ? pack2<T>(got, s[j + 16]) : pack2<T>(s[j], got);
-      }
-      // their buffer is free once the previous tile's product has read it
-      if (it > 0) wait(&sh.pv_done, it - 1);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<uint4*>(p_ptr + h * 128 + (((odd * 4 + c) ^ (h & 7)) << 4)) =
-            make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-      fence_async_shared();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full[it & 1]);
 
       if (at.last() || it == n - 1) {
-        wait(&sh.pv_done, it);
+        wait(&sh.pv_done[1], it);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         tc_fence_after();
         const bool whole = at.last() && segment_tile == 0;   // all of the row's tiles were here
@@ -475,9 +485,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   } else if (warp < 12) {
     // ---------------- producers ----------------
     const int half = (warp >> 1) & 1, turn_of = (warp - 4) >> 2, R0 = 32 * half + 16 * (warp & 1);
+    int segment = 0;
+    auto step = [&] {
+      if (at.last()) ++segment;
+      at.next(a);
+    };
     int pair = turn_of, turn = 0;                // tiles turn_of, turn_of + 2, ...; the number of pairs is even
     if (turn_of < n)
-      for (int i = 0; i < turn_of; ++i) at.next(a);
+      for (int i = 0; i < turn_of; ++i) step();
     auto slot_ahead = [&] {
       return lane < 16 ? slot_of(a, at.row, at.tile * static_cast<int64_t>(kTile) + R0 + lane) : -1;
     };
@@ -488,7 +503,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       if (lane == 0) {
         reinterpret_cast<volatile uint16_t*>(&sh.mask[pair])[R0 >> 4] = static_cast<uint16_t>(some);
         if (R0 == 0)
-          *reinterpret_cast<volatile uint32_t*>(&sh.flags[pair]) = (it == 0 || at.first() ? 1 : 0) | (at.last() ? 2 : 0);
+          *reinterpret_cast<volatile uint32_t*>(&sh.flags[pair]) =
+              (it == 0 || at.first() ? kFirst : 0) | (at.last() ? kLastOfRow : 0) |
+              (at.tile == at.tiles - 2 ? kBeforeLast : 0) | static_cast<uint32_t>(segment) * kSegment;
       }
       const char* src = slot >= 0 ? static_cast<const char*>(a.pool) + slot * a.pool_stride * 2 : nullptr;
       const RowCopy copy(kv_smem + pair * kChunks * kBlock, src, a.q, R0, lane);
@@ -497,8 +514,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       copy.template blocks<kEarly, kChunks>();
       cp_async_commit();
       if (it + 2 < n) {   // the next tile's slots arrive while this one's rows do
-        at.next(a);
-        at.next(a);
+        step();
+        step();
         slot = slot_ahead();
       }
       cp_async_wait<1>();
@@ -516,68 +533,87 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
       }
     }
     cp_async_wait_all();
-  } else if (warp == 12) {
-    // ---------------- scores ----------------
+  } else if (warp == 12 || warp == 14) {
+    // ---------------- scores: even tiles, odd tiles ----------------
     const uint32_t qk = idesc_16bit_f32(kBf16, kGroup, kTile, false, false), q_desc = desc_k(q_smem);
-    int rows_scored = 0, pair = 0, turn = 0, scored = 0;
-    for (int it = 0; it < n; ++it, ++scored) {
-      if (it >= 2 && !converged_wait(sh, a.status, &sh.p_full[it & 1], (it - 2) >> 1)) break;   // S is free again
+    const int mine = warp == 14;
+    int pair = mine, turn = 0, scored = -1;
+    // both warps take and give back every segment's queries, in order: also those of a
+    // segment whose only tile is the other warp's
+    int segment = 0;
+    bool held = false;
+    for (int it = mine; it < n; it += 2) {
+      if (it >= 2 && !converged_wait(sh, a.status, &sh.p_full[it & 1][1], (it - 2) >> 1)) break;   // S is free again
       if (!converged_wait(sh, a.status, &sh.full[2 * pair], turn)) break;
       const uint32_t flags = *reinterpret_cast<volatile uint32_t*>(&sh.flags[pair]);
-      if (__any_sync(0xffffffffu, flags & 1) && !converged_wait(sh, a.status, &sh.q_full, rows_scored++)) break;
+      bool ok = true;
+      for (const int now = static_cast<int>(flags / kSegment); segment < now && ok; ++segment) {
+        ok = converged_wait(sh, a.status, &sh.q_full, segment);
+        if (ok) umma_commit_elect(&sh.q_empty);
+      }
+      if (ok && !held) ok = held = converged_wait(sh, a.status, &sh.q_full, segment);
+      if (!ok) break;
       const uint32_t k_desc = desc_k(kv_smem + pair * kChunks * kBlock), d = tmem + kScoreCol + (it & 1) * kTile;
 #pragma unroll
       for (int c = 0; c < kEarly; ++c)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           umma_f16(d, q_desc + (c * kBlock + 32 * k) / 16, k_desc + (c * kBlock + 32 * k) / 16, qk, c + k > 0 ? 1u : 0u);
-      if (!converged_wait(sh, a.status, &sh.full[2 * pair + 1], turn)) {
-        umma_commit_elect(&sh.s_full[it & 1]);   // what was issued is waited for below
-        ++scored;
-        break;
+      const bool whole = converged_wait(sh, a.status, &sh.full[2 * pair + 1], turn);
+      if (whole) {
+#pragma unroll
+        for (int c = kEarly; c < kChunks; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(d, q_desc + (c * kBlock + 32 * k) / 16, k_desc + (c * kBlock + 32 * k) / 16, qk, 1u);
       }
-#pragma unroll
-      for (int c = kEarly; c < kChunks; ++c)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_f16(d, q_desc + (c * kBlock + 32 * k) / 16, k_desc + (c * kBlock + 32 * k) / 16, qk, c + k > 0 ? 1u : 0u);
       umma_commit_elect(&sh.s_full[it & 1]);
-      if (__any_sync(0xffffffffu, flags & 2)) umma_commit_elect(&sh.q_empty);
-      if (++pair == a.pairs) {
-        pair = 0;
+      scored = it;
+      if (!whole) break;
+      if (__any_sync(0xffffffffu, flags & (kLastOfRow | kBeforeLast))) {   // this warp's last tile of the row
+        umma_commit_elect(&sh.q_empty);
+        ++segment;
+        held = false;
+      }
+      pair += 2;
+      if (pair >= a.pairs) {
+        pair = mine;
         ++turn;
       }
     }
     // what was issued retires before the CTA ends
-    if (scored > 0) mbar_wait(&sh.s_full[(scored - 1) & 1], ((scored - 1) >> 1) & 1, &sh.zero, kWaitNs);
+    if (scored >= 0) mbar_wait(&sh.s_full[scored & 1], (scored >> 1) & 1, &sh.zero, kWaitNs);
   } else if (warp == 13) {
     // ---------------- output ----------------
     const uint32_t pv = idesc_16bit_f32(kBf16, 128, (heads + 15) & ~15, true, false), p_desc = desc_k(p_smem);
     int pair = 0, turn = 0, done = 0;
-    for (int it = 0; it < n; ++it, ++done) {
-      if (!converged_wait(sh, a.status, &sh.p_full[it & 1], it >> 1)) break;
-      const uint32_t more = (*reinterpret_cast<volatile uint32_t*>(&sh.flags[pair]) & 1) ^ 1;
-      const uint32_t v_desc = desc_mn(kv_smem + pair * kChunks * kBlock, kBlock);
+    for (int it = 0; it < n; ++it) {
+      bool ok = true;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
+        ok = ok && converged_wait(sh, a.status, &sh.p_full[it & 1][half], it >> 1);
+        if (!ok) break;
+        const uint32_t more = (*reinterpret_cast<volatile uint32_t*>(&sh.flags[pair]) & kFirst) ^ kFirst;
+        const uint32_t v_desc = desc_mn(kv_smem + pair * kChunks * kBlock, kBlock);
 #pragma unroll
         for (int t = 0; t < kOut; ++t)
 #pragma unroll
           for (int k = 2 * half; k < 2 * half + 2; ++k)
             umma_f16(tmem + t * 64, v_desc + (2 * t * kBlock + 2048 * k) / 16, p_desc + 32 * k / 16, pv, k > 0 ? 1u : more);
         umma_commit_elect(&sh.empty[2 * pair + half]);
+        umma_commit_elect(&sh.pv_done[half]);
+        ++done;
       }
-      umma_commit_elect(&sh.pv_done);
+      if (!ok) break;
       if (++pair == a.pairs) {
         pair = 0;
         ++turn;
       }
     }
-    if (done > 0) {
-      const int last = (done - 1) % a.pairs, phase = ((done - 1) / a.pairs) & 1;
-      mbar_wait(&sh.empty[2 * last], phase, &sh.zero, kWaitNs);
-      mbar_wait(&sh.empty[2 * last + 1], phase, &sh.zero, kWaitNs);
-      mbar_wait(&sh.pv_done, (done - 1) & 1, &sh.zero, kWaitNs);
+    if (done > 0) {   // halves done: the last one's commit follows all that was issued
+      const int it = (done - 1) >> 1, half = (done - 1) & 1;
+      mbar_wait(&sh.empty[2 * (it % a.pairs) + half], (it / a.pairs) & 1, &sh.zero, kWaitNs);
+      mbar_wait(&sh.pv_done[half], it & 1, &sh.zero, kWaitNs);
     }
   } else {
     // ---------------- queries ----------------
