@@ -2,6 +2,8 @@
 #include <cuda_fp8.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "attention.cuh"
 #include "sm100.cuh"
 
@@ -12,10 +14,12 @@ using namespace attn;
 using namespace sm100;
 
 // ---- store -------------------------------------------------------------------
-// One CTA per (touched page, head, K or V): the page's new tokens (four threads
-// a token, 32 values a thread, in registers), the largest magnitude over the CTA,
-// the scale, then the codes; the earlier tokens' codes are read only where the
-// scale rises.  Pure traffic: bytes of the new tokens in, half of them out.
+// One warp per (touched page, head, K or V): the page's new tokens (eight lanes a
+// token, 16 values a lane, the whole page in registers), the largest magnitude by
+// shuffles, the scale, then the codes; the earlier tokens' codes are read only
+// where the scale rises.  Pure traffic, bytes of the new tokens in and half of them
+// out, behind a chain of five dependent loads (request, its bounds, its page), which
+// is what a decode step's single tokens cost: so no barriers, many warps.
 //
 // The pages a request touches are found without a pass over the requests:
 // request r gets the units from base(r) = offsets[r] / 64 + 2 r on, at least as
@@ -57,92 +61,103 @@ __device__ __forceinline__ float2 values2(uint32_t two) {
   return __half22float2(__half2(h));
 }
 
+// The larger magnitudes of two pairs; of a NaN and a number the number.
 template <typename T>
-__global__ void __launch_bounds__(256) kv8_store_kernel(const __grid_constant__ StoreArgs a) {
-  __shared__ int64_t found;
-  __shared__ float part[8];
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int64_t u = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
-  if (tid < 32) {
-    // the last request r with base(r) <= u; base is strictly increasing
-    int64_t lo = 0, n = a.requests;
-    while (n > 1) {
-      const int64_t step = (n + 31) / 32, c = lo + lane * step;
-      const bool at = lane * step < n && clamped(a.offsets, c, a.tokens) / 64 + 2 * c <= u;
-      const int64_t k = max(__popc(__ballot_sync(0xffffffffu, at)) - 1, 0);
-      lo += k * step;
-      n = min(step, n - k * step);
-    }
-    if (lane == 0) found = lo;
+__device__ __forceinline__ uint32_t max_magnitudes(uint32_t a, uint32_t b) {
+  using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const Pair m = __hmax2(__habs2(*reinterpret_cast<Pair*>(&a)), __habs2(*reinterpret_cast<Pair*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128) kv8_store_kernel(const __grid_constant__ StoreArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t u = blockIdx.x, hz = static_cast<int64_t>(blockIdx.y) * 4 + (threadIdx.x >> 5);
+  if (hz >= 2 * a.heads) return;
+  const int64_t h = hz >> 1;
+  const int z = static_cast<int>(hz & 1);
+  // the last request r with base(r) <= u; base is strictly increasing
+  int64_t r = 0;
+  for (int64_t n = a.requests; n > 1;) {
+    const int64_t step = (n + 31) / 32, c = r + lane * step;
+    const bool at = lane * step < n && clamped(a.offsets, c, a.tokens) / 64 + 2 * c <= u;
+    const int64_t k = max(__popc(__ballot_sync(0xffffffffu, at)) - 1, 0);
+    r += k * step;
+    n = min(step, n - k * step);
   }
-  __syncthreads();
-  const int64_t r = found;
   const int64_t t0 = clamped(a.offsets, r, a.tokens), t1 = clamped(a.offsets, r + 1, a.tokens);
   const int64_t first = max(a.prefix[r], 0), end = first + (t1 - t0);
-  const int64_t n = u - (t0 / 64 + 2 * r);   // which of the request's pages (below 0: before the first request)
-  const int64_t i = first / 64 + n;          // the page's place in the table
-  if (t1 <= t0 || n < 0 || i * 64 >= end || i >= a.table_pages) return;
+  const int64_t nth = u - (t0 / 64 + 2 * r);   // which of the request's pages (below 0: before the first request)
+  const int64_t i = first / 64 + nth;          // the page's place in the table
+  if (t1 <= t0 || nth < 0 || i * 64 >= end || i >= a.table_pages) return;
   const int64_t page = a.table[r * a.table_stride + i];
   if (page < 0 || page >= a.pages) return;
 
-  const int64_t pos = i * 64 + (tid >> 2);
-  const bool fresh = pos >= first && pos < end;
-  const int d0 = (tid & 3) * 8;   // 16-byte chunks (tid & 3), + 4, + 8, + 12 of the row
-  uint4 raw[4];
-  float most = 0.0f;
-  if (fresh) {
-    const T* x = static_cast<const T*>(a.x[z]) + (t0 + pos - first) * a.s0[z] + h * a.s1[z];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) raw[c] = *reinterpret_cast<const uint4*>(x + d0 + 32 * c);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = to_float2<T>(w[e]);
-        most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));   // a NaN counts for nothing
-      }
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  if (lane == 0) part[tid >> 5] = most;
-  __syncthreads();
-  most = part[0];
-#pragma unroll
-  for (int w = 1; w < 8; ++w) most = fmaxf(most, part[w]);
+  // the page's tokens [lo, hi) are new, those before lo earlier ones
+  const int lo = static_cast<int>(max(first - i * 64, int64_t(0))), hi = static_cast<int>(min(end - i * 64, int64_t(64)));
+  const int sub = lane >> 3, d0 = (lane & 7) * 16;   // of token 4 k + sub: values d0 .. d0 + 15
+  const T* x = static_cast<const T*>(a.x[z]) + (t0 + i * 64 - first + sub) * a.s0[z] + h * a.s1[z] + d0;
+  const int64_t four = 4 * a.s0[z];
   float* const sp = a.scale[z] + page * a.heads + h;
-  float now = scale_for(most);
-  const bool begun = first > i * 64;
-  const float old = begun ? *sp : now;
-  now = begun ? fmaxf(now, old) : now;
-  __syncthreads();   // everyone has the former scale
-  if (tid == 0) *sp = now;
-
-  uint8_t* const row = a.cache[z] + ((page * a.heads + h) * 64 + (tid >> 2)) * 128;
-  if (fresh) {
-    const float inv = 1.0f / now;   // a power of two
+  const float former = *sp;
+  uint4 raw[16][2];
+  const uint4 none = make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const float2 f0 = to_float2<T>(raw[c].x), f1 = to_float2<T>(raw[c].y);
-      const float2 f2 = to_float2<T>(raw[c].z), f3 = to_float2<T>(raw[c].w);
-      *reinterpret_cast<uint2*>(row + d0 + 32 * c) =
-          make_uint2(codes4(f0.x * inv, f0.y * inv, f1.x * inv, f1.y * inv),
-                     codes4(f2.x * inv, f2.y * inv, f3.x * inv, f3.y * inv));
+  for (int k = 0; k < 16; ++k) {
+    const int t = 4 * k + sub;
+    const bool fresh = t >= lo && t < hi;
+    raw[k][0] = raw[k][1] = none;
+    if (fresh) {
+      raw[k][0] = *reinterpret_cast<const uint4*>(x);
+      raw[k][1] = *reinterpret_cast<const uint4*>(x + 8);
     }
-  } else if (pos < first && now != old) {
-    const float ratio = old / now;
-    uint4* const p = reinterpret_cast<uint4*>(row + (tid & 3) * 32);
+    x += four;
+  }
+  uint32_t tops[2] = {0, 0};     // pairs; a NaN counts for nothing
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      uint4 v = p[c];
+      tops[c] = max_magnitudes<T>(tops[c], max_magnitudes<T>(raw[k][c].x, raw[k][c].y));
+      tops[c] = max_magnitudes<T>(tops[c], max_magnitudes<T>(raw[k][c].z, raw[k][c].w));
+    }
+  const float2 top = to_float2<T>(max_magnitudes<T>(tops[0], tops[1]));
+  float most = fmaxf(top.x, top.y);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  float now = scale_for(most);
+  const float old = lo > 0 ? former : now;
+  now = lo > 0 ? fmaxf(now, old) : now;
+  if (lane == 0) *sp = now;
+
+  uint8_t* const rows = a.cache[z] + (page * a.heads + h) * 64 * 128 + d0, * const own = rows + sub * 128;
+  const float inv = 1.0f / now;   // a power of two
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int t = 4 * k + sub;
+    if (t < lo || t >= hi) continue;
+    uint32_t w[4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float2 f0 = to_float2<T>(raw[k][c].x), f1 = to_float2<T>(raw[k][c].y);
+      const float2 f2 = to_float2<T>(raw[k][c].z), f3 = to_float2<T>(raw[k][c].w);
+      w[2 * c] = codes4(f0.x * inv, f0.y * inv, f1.x * inv, f1.y * inv);
+      w[2 * c + 1] = codes4(f2.x * inv, f2.y * inv, f3.x * inv, f3.y * inv);
+    }
+    *reinterpret_cast<uint4*>(own + k * 512) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (now != old) {               // the same in all lanes
+    const float ratio = old / now;
+    for (int t = sub; t < lo; t += 4) {
+      uint4* const p = reinterpret_cast<uint4*>(rows + t * 128);
+      const uint4 v = *p;
       uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 lo = values2(w[e]), hi = values2(w[e] >> 16);
-        w[e] = codes4(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
+        const float2 f = values2(w[e]), g = values2(w[e] >> 16);
+        w[e] = codes4(f.x * ratio, f.y * ratio, g.x * ratio, g.y * ratio);
       }
-      p[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      *p = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
@@ -592,17 +607,29 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   }
 }
 
-// Joins the parts of the segments that lie in several ranges.  Grid x: the segment in
-// which range x begins, if x is the first range to begin inside it; the parts in the
-// order of the ranges.  Range y's part is its first (slot 0) unless the range begins
-// in an earlier segment (then its last, slot 1); a range may be empty.  kShare warps
-// share the parts of one head.
+// Joins the parts of the segments that lie in several ranges, in the order of the
+// ranges.  Range y's part is its first (slot 0) unless the range begins in an earlier
+// segment (then its last, slot 1); a range may be empty.  kShare warps share the parts
+// of one head.  Grid x: with kShare = 1 the segment in which range x + 1 begins, if
+// that is the first range to begin inside it (many segments of a few parts); else
+// the segment x (a few of many parts).
 template <typename T, int kTiles, int kShare>
 __global__ void __launch_bounds__(kShare == 1 ? 128 : 32 * kShare) kv8_join_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int kHeads = 8 * kTiles;
   __shared__ float4 sums[kShare][32];
   __shared__ float ls[kShare];
-  const int x = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int x = blockIdx.x + 1;
+  if constexpr (kShare > 1) {
+    __shared__ int found;
+    if (threadIdx.x == 0) found = kMaxRanges;
+    __syncthreads();
+    for (int i = threadIdx.x + 1; i < a.ranges; i += 32 * kShare)
+      if (a.where[4 * i] == blockIdx.x && a.where[4 * i + 3] > a.where[4 * i + 1]) atomicMin(&found, i);
+    __syncthreads();
+    x = found;
+    if (x == kMaxRanges) return;
+  }
   const int64_t first = a.where[4 * x + 1], begin = a.where[4 * x + 3], before = a.where[4 * x - 1];
   if (begin == first || before > first) return;
   const int64_t place = a.where[4 * x], end = first + a.where[4 * x + 2];
@@ -678,7 +705,8 @@ void launch_attend(const CUtensorMap& k_map, const CUtensorMap& v_map, const Att
   if (a.ranges == 1) return;
   const unsigned cuts = static_cast<unsigned>(a.ranges - 1), heads = 8 * kTiles;
   if (a.ranges >= 16 * a.rows * a.segments)   // many parts a segment
-    launch_kernel_prio(LaunchPriority::kDefault, kv8_join_kernel<T, kTiles, 16>, dim3(cuts, heads), dim3(512), 0, s, a);
+    launch_kernel_prio(LaunchPriority::kDefault, kv8_join_kernel<T, kTiles, 16>,
+                       dim3(static_cast<unsigned>(a.rows * a.segments), heads), dim3(512), 0, s, a);
   else
     launch_kernel_prio(LaunchPriority::kDefault, kv8_join_kernel<T, kTiles, 1>, dim3(cuts, heads / 4), dim3(128), 0, s, a);
 }
@@ -731,11 +759,11 @@ extern "C" int v1x_kv8_store(uint8_t* k_cache, float* k_scale, uint8_t* v_cache,
   V1X_CHECK_ARG(k_cache && k_scale && v_cache && v_scale && k && v && table && prefix && offsets, "kv8_store: NULL argument");
   StoreArgs a{{k_cache, v_cache}, {k_scale, v_scale}, {k, v}, {ks0, vs0}, {ks1, vs1}, pages, heads, tokens,
               table, table_stride, table_pages, prefix, offsets, requests};
-  const dim3 grid(static_cast<unsigned>(tokens / 64 + 2 * requests), static_cast<unsigned>(heads), 2);
+  const dim3 grid(static_cast<unsigned>(tokens / 64 + 2 * requests), static_cast<unsigned>((2 * heads + 3) / 4));
   if (dtype == 1)
-    launch_kernel_prio(LaunchPriority::kDefault, kv8_store_kernel<__nv_bfloat16>, grid, dim3(256), 0, as_stream(stream), a);
+    launch_kernel_prio(LaunchPriority::kDefault, kv8_store_kernel<__nv_bfloat16>, grid, dim3(128), 0, as_stream(stream), a);
   else
-    launch_kernel_prio(LaunchPriority::kDefault, kv8_store_kernel<__half>, grid, dim3(256), 0, as_stream(stream), a);
+    launch_kernel_prio(LaunchPriority::kDefault, kv8_store_kernel<__half>, grid, dim3(128), 0, as_stream(stream), a);
   return launch_status("v1x_kv8_store");
 }
 
