@@ -618,6 +618,7 @@ __global__ void __launch_bounds__(kShare == 1 ? 128 : 32 * kShare) kv8_join_kern
   constexpr int kHeads = 8 * kTiles;
   __shared__ float4 sums[kShare][32];
   __shared__ float ls[kShare];
+  wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int x = blockIdx.x + 1;
   if constexpr (kShare > 1) {
@@ -705,10 +706,9 @@ void launch_attend(const CUtensorMap& k_map, const CUtensorMap& v_map, const Att
   if (a.ranges == 1) return;
   const unsigned cuts = static_cast<unsigned>(a.ranges - 1), heads = 8 * kTiles;
   if (a.ranges >= 16 * a.rows * a.segments)   // many parts a segment
-    launch_kernel_prio(LaunchPriority::kDefault, kv8_join_kernel<T, kTiles, 16>,
-                       dim3(static_cast<unsigned>(a.rows * a.segments), heads), dim3(512), 0, s, a);
+    launch_join(kv8_join_kernel<T, kTiles, 16>, dim3(static_cast<unsigned>(a.rows * a.segments), heads), dim3(512), s, a);
   else
-    launch_kernel_prio(LaunchPriority::kDefault, kv8_join_kernel<T, kTiles, 1>, dim3(cuts, heads / 4), dim3(128), 0, s, a);
+    launch_join(kv8_join_kernel<T, kTiles, 1>, dim3(cuts, heads / 4), dim3(128), s, a);
 }
 
 // Rows of 128 codes, 64 (a page and head) a box, 128-byte swizzle.

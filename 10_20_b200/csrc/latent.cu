@@ -657,6 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
 template <typename T, int kLatent, int kWarps>
 __global__ void __launch_bounds__(128) latent_join_kernel(const __grid_constant__ LatentArgs a) {
   constexpr int kPer = kWarps == 1 ? kLatent / 128 : 1;   // 16-byte pieces of a lane
+  wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = kWarps == 1 ? static_cast<int>(blockIdx.y) * 4 + warp : static_cast<int>(blockIdx.y);
   int x = blockIdx.x + 1;
@@ -772,11 +773,9 @@ void launch(LatentArgs a, bool join, cudaStream_t s) {
   if (!join) return;
   const unsigned cuts = static_cast<unsigned>(a.ranges - 1), heads = static_cast<unsigned>(a.heads);
   if (a.ranges >= 8 * a.rows)
-    launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<T, kLatent, 4>, dim3(static_cast<unsigned>(a.rows), heads, kLatent / 128),
-                       dim3(128), 0, s, a);
+    launch_join(latent_join_kernel<T, kLatent, 4>, dim3(static_cast<unsigned>(a.rows), heads, kLatent / 128), dim3(128), s, a);
   else
-    launch_kernel_prio(LaunchPriority::kDefault, latent_join_kernel<T, kLatent, 1>, dim3(cuts, (heads + 3) / 4),
-                       dim3(128), 0, s, a);
+    launch_join(latent_join_kernel<T, kLatent, 1>, dim3(cuts, (heads + 3) / 4), dim3(128), s, a);
 }
 
 template <typename T>
