@@ -416,10 +416,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
         T* const out = static_cast<T*>(a.out) + (static_cast<int64_t>(at.row) * a.heads + group * kGroup) * kLatent;
         const int d = warp * 32 + lane;
         if (whole) {
-          // 16 heads x 128 columns at a time through a half of the weights' buffer (free:
-          // the last product has read it), so that a head's 256 bytes are written as one
-          // piece; the halves alternate, one barrier a step
-          int side = 0;
+          // 32 heads x 32 columns at a time through the warp's quarter of the weights'
+          // buffer (free: the last product has read it), so that a lane writes 16 bytes
+          // of a head and four of them its 64
+          uint8_t* const mine_p = p_ptr + warp * (kBlock / 4);
+          uint16_t* const put = reinterpret_cast<uint16_t*>(mine_p) + lane;
+          T* const to = out + warp * 32 + (lane & 3) * 8;
 #pragma unroll 1
           for (int t = 0; t < kOut; ++t)
 #pragma unroll 1
@@ -428,29 +430,23 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
               tmem_ld32(tmem + quarter + t * 64 + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int b = 0; b < 32; b += 16) {
-                uint8_t* const buffer = p_ptr + side * (kBlock / 2);
-                uint16_t* const to = reinterpret_cast<uint16_t*>(buffer) + d;
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                  const float4 f = *reinterpret_cast<const float4*>(&sh.factor[c + b + j]);
-                  const uint32_t u = pack2<T>(__uint_as_float(o[b + j]) * f.x, __uint_as_float(o[b + j + 1]) * f.y);
-                  const uint32_t v = pack2<T>(__uint_as_float(o[b + j + 2]) * f.z, __uint_as_float(o[b + j + 3]) * f.w);
-                  to[j * 128] = static_cast<uint16_t>(u);
-                  to[(j + 1) * 128] = static_cast<uint16_t>(u >> 16);
-                  to[(j + 2) * 128] = static_cast<uint16_t>(v);
-                  to[(j + 3) * 128] = static_cast<uint16_t>(v >> 16);
-                }
-                sync_128();
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  const int hh = 8 * i + (tid >> 4), e = (tid & 15) * 8;
-                  if (c + b + hh < heads)
-                    *reinterpret_cast<uint4*>(out + (c + b + hh) * kLatent + t * 128 + e) =
-                        *reinterpret_cast<const uint4*>(buffer + hh * 256 + e * 2);
-                }
-                side ^= 1;
+              for (int j = 0; j < 32; j += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(&sh.factor[c + j]);
+                const uint32_t u = pack2<T>(__uint_as_float(o[j]) * f.x, __uint_as_float(o[j + 1]) * f.y);
+                const uint32_t v = pack2<T>(__uint_as_float(o[j + 2]) * f.z, __uint_as_float(o[j + 3]) * f.w);
+                put[j * 32] = static_cast<uint16_t>(u);
+                put[(j + 1) * 32] = static_cast<uint16_t>(u >> 16);
+                put[(j + 2) * 32] = static_cast<uint16_t>(v);
+                put[(j + 3) * 32] = static_cast<uint16_t>(v >> 16);
               }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int hh = c + 8 * i + (lane >> 2);
+                const uint4 v = *reinterpret_cast<const uint4*>(mine_p + i * 512 + lane * 16);
+                if (hh < heads) *reinterpret_cast<uint4*>(to + hh * kLatent + t * 128) = v;
+              }
+              __syncwarp();
             }
         } else {
 #pragma unroll 1
