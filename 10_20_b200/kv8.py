@@ -44,7 +44,8 @@ def _cache(k_cache, k_scale, v_cache, v_scale):
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(rows, heads, kv_heads, table_pages) -> int:
+def workspace_bytes(rows, heads, kv_heads, table_pages) -> int:
+    """Device bytes ``attend`` needs besides its outputs (0: one kernel)."""
     return _lib.lib().v1x_kv8_attend_workspace(rows, heads, kv_heads, table_pages)
 
 
@@ -102,7 +103,7 @@ def attend(q, k_cache, k_scale, v_cache, v_scale, table, lens, scale, out=None, 
     out, lse = _outputs(q, (rows, heads, 128), out, lse)
     if rows == 0:
         return out, lse
-    size = _workspace_bytes(rows, heads, kv_heads, table.shape[1])
+    size = workspace_bytes(rows, heads, kv_heads, table.shape[1])
     work = q.new_empty(size, dtype=torch.uint8) if size else None
     _lib.call("v1x_kv8_attend", q.data_ptr(), _step(q, 0), _step(q, 1), k_cache.data_ptr(), k_scale.data_ptr(),
               v_cache.data_ptr(), v_scale.data_ptr(), pages, kv_heads, table.data_ptr(), _step(table, 0),

@@ -84,7 +84,9 @@ def _outputs(q, shape, out, lse):
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(rows, heads, count, latent, equal) -> int:
+def workspace_bytes(rows, heads, count, latent, equal) -> int:
+    """Device bytes an absorbed call needs besides its outputs (0: one kernel, no
+    parts to join); equal: every row has ``count`` places (``attend_slots``)."""
     return _lib.lib().v1x_latent_attention_workspace(rows, heads, count, latent, equal)
 
 
@@ -106,7 +108,7 @@ def _absorbed(q, pool, request_slots, index, count, lens, scale, latent, out, ls
     out, lse = _outputs(q, (rows, heads, latent), out, lse)
     if rows == 0:
         return out, lse
-    size = _workspace_bytes(rows, heads, count, latent, lens is None)
+    size = workspace_bytes(rows, heads, count, latent, lens is None)
     work = q.new_empty(size, dtype=torch.uint8) if size else None
     _lib.call("v1x_latent_attention", q.data_ptr(), _step(q, 0), _step(q, 1), pool.data_ptr(), pool.shape[0],
               _step(pool, 0), ptr(request_slots), 0 if request_slots is None else request_slots.shape[0],

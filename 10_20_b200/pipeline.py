@@ -35,7 +35,7 @@ from . import _lib
 from . import kernels as K
 from . import query_fused, scoring
 from .gather import _gather_impl
-from .latent_attention import attend_slots
+from .latent_attention import attend_slots, workspace_bytes
 from .sharding import row_bytes
 
 
@@ -260,8 +260,12 @@ class SelectionStep:
     # -- accounting ----------------------------------------------------------
     def launches(self) -> int:
         """Kernels one run() launches (centre scoring + selection, or the five
-        operators; + the gather; + the attention and its join)."""
-        return (2 if self.fused_select else 5) + (1 if self.gather else 0) + (2 if self.attention is not None else 0)
+        operators; + the gather; + the attention and, where rows lie in several
+        CTAs' ranges, its join)."""
+        n = (2 if self.fused_select else 5) + (1 if self.gather else 0)
+        if self.attention is not None:
+            n += 2 if workspace_bytes(self.case.B, self.attention[0].shape[1], self.case.topk, 512, True) else 1
+        return n
 
     def algorithmic_bytes(self) -> dict:
         """Compulsory bytes of one step, each input byte once, each output once

@@ -624,4 +624,4 @@ def test_selection_step_attends():
     step.replay()
     want = L.attend_slots(q, case.latent, None, step.physical, 0.07)
     assert torch.equal(step.attended[0], want[0]) and torch.equal(step.attended[1], want[1])
-    assert step.launches() >= 3
+    assert step.launches() == 4      # two of the selection, the attention of three rows and its join
