@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   } else if (warp == 13) {
     // ---------------- output ----------------
     const uint32_t pv = idesc_16bit_f32(kBf16, 128, (heads + 15) & ~15, true, false), p_desc = desc_k(p_smem);
-    int pair = 0, turn = 0, done = 0;
+    int pair = 0, done = 0;
     for (int it = 0; it < n; ++it) {
       bool ok = true;
 #pragma unroll
@@ -607,10 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
         ++done;
       }
       if (!ok) break;
-      if (++pair == a.pairs) {
-        pair = 0;
-        ++turn;
-      }
+      if (++pair == a.pairs) pair = 0;
     }
     if (done > 0) {   // halves done: the last one's commit follows all that was issued
       const int it = (done - 1) >> 1, half = (done - 1) & 1;

@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(pending);
     };
-    int slot = 0, turn = 0;
+    int slot = 0, turn = 0, boxes[kSlots] = {-1, -1, -1};   // boxes: the turn of a slot's last TMA load
     for (int u = 0; u < 2 * n; ++u) {
       const int j = u >> 1, rope = j % kRopeSlots;
       const bool keys = (u & 1) == 0;
@@ -407,6 +407,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i)
+          if (i == slot) boxes[i] = turn;
         if (++slot == kSlots) {
           slot = 0;
           ++turn;
@@ -429,6 +432,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     cp_async_wait_all();
     if (pending) report();
+    if (*reinterpret_cast<volatile int*>(&sh.abort) && half == 0)   // boxes that are under way land before the CTA ends
+      for (int i = 0; i < kSlots; ++i)
+        if (boxes[i] >= 0) mbar_wait(&sh.full[i], boxes[i] & 1, &sh.zero, kWaitNs);
   }
   __syncthreads();
   if (warp == 8) {
@@ -515,8 +521,9 @@ extern "C" int v1x_prompt_attention(const void* q, int64_t qs0, int64_t qs1, con
                 "prompt_attention: q, k, k_rope, v and out rows must be 16-byte aligned");
   if (tokens == 0 || requests == 0) return V1X_OK;
   V1X_CHECK_ARG(q && out && lse && offsets && kv_offsets && ((k && v) || keys == 0), "prompt_attention: NULL argument");
-  // a masked score, -inf, has to stay -inf under the scale
-  const float magnitude = scale == 0 ? 1e-30f : (scale < 0 ? -scale : scale) * kLog2e;
+  // a masked score, -inf, has to stay -inf under the scale, so that is never 0
+  float magnitude = (scale < 0 ? -scale : scale) * kLog2e;
+  if (magnitude < 1e-30f) magnitude = 1e-30f;
   const PromptArgs a{q,    k,     k_rope, v, qs0, qs1, ks0, ks1, krs0, vs0, vs1, offsets, kv_offsets, requests, tokens,
                      keys, heads, magnitude, scale < 0 ? 1 : 0, out, lse, status, 0};
   cudaStream_t s = as_stream(stream);

@@ -155,7 +155,9 @@ def attend_prompt(q, k, k_rope, v, offsets, scale, kv_offsets=None, out=None, ls
     (bfloat16 / float16), unit inner stride, rows 16-byte aligned -- views of
     one projection's output or of pool rows are taken as they are.  offsets and
     kv_offsets: int32 [requests + 1], non-decreasing, within the tokens.  Rows
-    of q that no request covers are left as they are in out and lse."""
+    of q that no request covers are left as they are in out and lse.  A NaN or an
+    infinity among a request's values also reaches queries that come before it
+    (0 times it is NaN); other requests' keys and values are never read."""
     code = _DTYPES.get(q.dtype)
     require(code is not None and q.dim() == 3, "q: [tokens, heads, 128 + dr] bfloat16 or float16")
     tokens, heads, width = q.shape
