@@ -30,6 +30,29 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// ---- two floats in one 64-bit register, one instruction for both ----------------
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 two(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 both(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // two floats rounded to nearest even, the first in the low half
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
