@@ -249,12 +249,18 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 // 8 kTiles query heads at a time
 template <typename T, int kTiles>
 __global__ void __launch_bounds__(kWarps * 32, 1)
     kv8_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                       const __grid_constant__ AttendArgs a) {
-  constexpr int kHeads = 8 * kTiles;
+  constexpr int kHeads = 8 * kTiles, kPasses = kTiles;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   AttendShared& sh = *reinterpret_cast<AttendShared*>(base + kWarps * kRing * kPageBytes8);
@@ -512,45 +518,62 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       }
       arrived(vslot);
       const uint32_t v = ring + vslot * kPageBytes8;
-      float acc[kTiles][8][4];
+      // a lane's 16 columns in kPasses parts: two tiles' sums of all 16 would not fit the
+      // registers beside the rest
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
+      for (int pass = 0; pass < kPasses; ++pass) {
+        float acc[kTiles][8 / kPasses][4];
 #pragma unroll
-        for (int d = 0; d < 8; ++d)
+        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][d][i] = 0.0f;
+          for (int d = 0; d < 8 / kPasses; ++d)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // tokens 16 j + 2 tig, + 1, + 8, + 9; columns 16 g .. 16 g + 15
-        uint32_t x4[4][4];
+            for (int i = 0; i < 4; ++i) acc[t][d][i] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int token = 16 * j + 2 * tig + (i & 1) + 8 * (i >> 1);
-          uint4 u = lds128(v + token * 128 + ((g ^ ((2 * tig + (i & 1)) & 7)) << 4));
-          if (token >= left) u = make_uint4(0, 0, 0, 0);   // places behind the last token may hold NaN codes
-          x4[i][0] = u.x;
-          x4[i][1] = u.y;
-          x4[i][2] = u.z;
-          x4[i][3] = u.w;
+        for (int j = 0; j < 4; ++j) {
+          // tokens 16 j + 2 tig, + 1, + 8, + 9; columns 16 g .. 16 g + 15
+          uint32_t x4[4][4 / kPasses];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int token = 16 * j + 2 * tig + (i & 1) + 8 * (i >> 1);
+            const uint32_t at = v + token * 128 + ((g ^ ((2 * tig + (i & 1)) & 7)) << 4);
+            // places behind the last token may hold NaN codes
+            if constexpr (kPasses == 1) {
+              uint4 u = lds128(at);
+              if (token >= left) u = make_uint4(0, 0, 0, 0);
+              x4[i][0] = u.x;
+              x4[i][1] = u.y;
+              x4[i][2] = u.z;
+              x4[i][3] = u.w;
+            } else {
+              uint2 u = lds64(at + 8 * pass);
+              if (token >= left) u = make_uint2(0, 0);
+              x4[i][0] = u.x;
+              x4[i][1] = u.y;
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < 4 / kPasses; ++w)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {      // columns 4 w + 2 y, + 1 of the part: rows g and g + 8 of block 2 w + y
+              const uint32_t lo = __byte_perm(x4[0][w], x4[1][w], y ? 0x7362 : 0x5140);
+              const uint32_t hi = __byte_perm(x4[2][w], x4[3][w], y ? 0x7362 : 0x5140);
+              const uint32_t a0 = half2_of(lo), a1 = half2_of_high(lo), a2 = half2_of(hi), a3 = half2_of_high(hi);
+#pragma unroll
+              for (int t = 0; t < kTiles; ++t) mma16816(acc[t][2 * w + y], a0, a1, a2, a3, p[t][2 * j], p[t][2 * j + 1]);
+            }
         }
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {        // columns 4 w + 2 y, + 1 of the lane's 16: rows g and g + 8 of block 2 w + y
-            const uint32_t lo = __byte_perm(x4[0][w], x4[1][w], y ? 0x7362 : 0x5140);
-            const uint32_t hi = __byte_perm(x4[2][w], x4[3][w], y ? 0x7362 : 0x5140);
-            const uint32_t a0 = half2_of(lo), a1 = half2_of_high(lo), a2 = half2_of(hi), a3 = half2_of_high(hi);
+          for (int d = 0; d < 8 / kPasses; ++d)
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t) mma16816(acc[t][2 * w + y], a0, a1, a2, a3, p[t][2 * j], p[t][2 * j + 1]);
-          }
+            for (int i = 0; i < 4; ++i) {
+              float& e = o[t][pass * (8 / kPasses) + d][i];
+              e = fmaf(acc[t][d][i], cur.vs, e);
+            }
       }
       __syncwarp();
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[t][d][i] = fmaf(acc[t][d][i], cur.vs, o[t][d][i]);
     } else {
       load(&v_map, slot, nxt.at);
     }
