@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(128) kv8_store_kernel(const __grid_constant__ 
 //     of a key's 128 dims lane tig takes 32 tig .. 32 tig + 31, of the values' columns
 //     lane g takes 16 g .. 16 g + 15; with the buffers' 128-byte swizzle every 16-byte
 //     read is free of conflicts;
-// 64 rows of 1-16 K tokens, 32 heads over 4: 110 us, 5.2 TB/s (the kernel 98, the join
-// the rest); one row of 4097 tokens 13 us.
+// 64 rows of 1-16 K tokens, 32 heads over 4: 103 us, 5.5 TB/s (the join about 8 of them);
+// one row of 4097 tokens 13 us.
 //   * the query is held in f16 under a power of two per head that puts its largest
 //     value in [1, 2); the weights are rounded to f16 once, sums stay in 32 bits; a
 //     page's output is added under its value scale in 32 bits, so scales of any size
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const int64_t x = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
   const int64_t per = all >> 31 ? all / a.ranges : static_cast<uint32_t>(all) / static_cast<uint32_t>(a.ranges);
   const int64_t extra = all - per * a.ranges;
-  const int64_t t0 = x * per + min(x, extra), n = x < a.ranges ? per + (x < extra ? 1 : 0) : 0;
+  const int64_t t0 = x * per + min(x, extra), pages_mine = x < a.ranges ? per + (x < extra ? 1 : 0) : 0;
   int64_t row = 0, pages = 1, page = 0, segment = 0, first = 0;
   if (all > 0 && x < a.ranges) {
     int lo = 0;   // the last thread whose rows begin at or before t0 (those behind it with the same prefix are empty)
@@ -313,8 +313,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   }
 
   // ---- the walk ---------------------------------------------------------------------
+  const int n = static_cast<int>(pages_mine);
   struct Place {
-    int64_t row, segment, page, pages;
+    int row, segment, page, pages;
   };
   auto next = [&](Place& p) {
     if (++p.page < p.pages) return;
@@ -323,19 +324,19 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     p.segment = 0;
     do {
       ++p.row;
-      p.pages = p.row < a.rows ? row_pages(a, p.row) : 1;
+      p.pages = p.row < a.rows ? static_cast<int>(row_pages(a, p.row)) : 1;
     } while (p.pages == 0);
   };
   // a page of the cache and its scales; block < 0: none
   struct Block {
-    int64_t at;
+    int at;
     float ks, vs;
   };
   auto block_of = [&](const Place& p) {
     Block b{-1, 0.0f, 0.0f};
-    const int64_t id = a.table[p.row * a.table_stride + p.page];
-    if (id >= 0 && id < a.pages) {
-      b.at = id * a.kv_heads + p.segment / a.groups;
+    const int id = a.table[p.row * a.table_stride + p.page];
+    if (id >= 0 && id < a.pages) {             // pages * kv_heads < 2^25
+      b.at = id * static_cast<int>(a.kv_heads) + p.segment / a.groups;
       b.ks = a.ks[b.at];
       b.vs = a.vs[b.at];
     }
@@ -344,12 +345,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const uint32_t ring = smem_u32(base + warp * kRing * kPageBytes8);
   uint64_t* const full = sh.full[warp];
   uint32_t phases = 0, issued = 0;             // per buffer: the phase that the next wait is for; a load is in flight
-  auto load = [&](const CUtensorMap* map, int slot, int64_t at) {
+  auto load = [&](const CUtensorMap* map, int slot, int at) {
     if (at < 0) return;
     issued |= 1u << slot;
     if (lane == 0) {
       mbar_arrive_expect_tx(&full[slot], kPageBytes8);
-      tma_load_2d(base + (warp * kRing + slot) * kPageBytes8, map, &full[slot], 0, static_cast<int>(at * 64));
+      tma_load_2d(base + (warp * kRing + slot) * kPageBytes8, map, &full[slot], 0, at * 64);
     }
   };
   bool ok = true;
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     issued &= ~(1u << slot);
   };
 
-  Place now{row, segment, page, pages}, ahead = now;   // ahead: the page whose block was looked up last
+  Place now{static_cast<int>(row), static_cast<int>(segment), static_cast<int>(page), static_cast<int>(pages)}, ahead = now;   // ahead: the page whose block was looked up last
   Block cur{-1, 0, 0}, nxt{-1, 0, 0};
   if (n > 0) {
     cur = block_of(ahead);
@@ -379,12 +380,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   float qscale[kTiles][2];                     // of the two heads of this lane's columns, scale and base 2 included
   float o[kTiles][8][4], m[kTiles][2], l[kTiles][2];
   bool fresh = true;
-  int64_t parts = 0;
+  int parts = 0;
   int slot = 0;                                // of the page's keys; its values follow
-  for (int64_t it = 0; it < n && ok; ++it) {
-    const int kv = static_cast<int>(now.segment / a.groups), group = static_cast<int>(now.segment % a.groups);
+  for (int it = 0; it < n && ok; ++it) {
+    const int kv = now.segment / a.groups, group = now.segment % a.groups;
     const int heads = min(kHeads, a.per_kv - group * kHeads);
-    const int64_t head0 = static_cast<int64_t>(kv) * a.per_kv + group * kHeads;
+    const int head0 = kv * a.per_kv + group * kHeads;
     if (fresh) {
       fresh = false;
 #pragma unroll
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         for (int c = 0; c < 4; ++c) {
           raw[c] = make_uint4(0, 0, 0, 0);
           if (hh < heads)
-            raw[c] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + now.row * a.qs0 + (head0 + hh) * a.qs1 +
+            raw[c] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + now.row * a.qs0 + static_cast<int64_t>(head0 + hh) * a.qs1 +
                                                      32 * tig + 8 * c);
           const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       next(ahead);
       far = block_of(ahead);
     }
-    const int left = static_cast<int>(min(static_cast<int64_t>(a.lens[now.row]) - now.page * 64, int64_t(64)));
+    const int left = min(a.lens[now.row] - now.page * 64, 64);   // page < pages: no overflow
     const int vslot = slot + 1 == kRing ? 0 : slot + 1;
     uint32_t p[kTiles][8];                     // weights as the second product's operand
     if (cur.at >= 0) {
@@ -451,21 +452,27 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
           for (int i = 0; i < 4; ++i) s[t][j][i] = 0.0f;
       arrived(slot);
       const uint32_t k = ring + slot * kPageBytes8;
+      // token tiles j innermost: their sums are independent, one's next step waits 20 cycles
+      const uint32_t r0 = k + g * 128;         // tokens 16 j + g, + 8: the same row & 7
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t r0 = k + (16 * j + g) * 128, r1 = r0 + 8 * 128;   // tokens 16 j + g, + 8: the same row & 7
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t at = r0 + static_cast<uint32_t>(((2 * tig + c) ^ g) << 4);
+        uint4 u[4], v[4];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t at = static_cast<uint32_t>(((2 * tig + c) ^ g) << 4);
-          const uint4 u = lds128(r0 + at), v = lds128(r1 + at);
-          const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+        for (int j = 0; j < 4; ++j) {
+          u[j] = lds128(at + j * 2048);
+          v[j] = lds128(at + j * 2048 + 1024);
+        }
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t a0 = half2_of(uw[w]), a1 = half2_of(vw[w]), a2 = half2_of_high(uw[w]), a3 = half2_of_high(vw[w]);
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t uw = w == 0 ? u[j].x : w == 1 ? u[j].y : w == 2 ? u[j].z : u[j].w;
+            const uint32_t vw = w == 0 ? v[j].x : w == 1 ? v[j].y : w == 2 ? v[j].z : v[j].w;
+            const uint32_t a0 = half2_of(uw), a1 = half2_of(vw), a2 = half2_of_high(uw), a3 = half2_of_high(vw);
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) mma16816(s[t][j], a0, a1, a2, a3, q[t][4 * c + w][0], q[t][4 * c + w][1]);
           }
-        }
       }
       __syncwarp();
       load(&v_map, slot, nxt.at);              // the keys' buffer is free: the next page's values
@@ -594,14 +601,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
           if (hh >= heads) continue;
           const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
           if (whole) {
-            T* const out = static_cast<T*>(a.out) + (now.row * a.heads + head0 + hh) * 128 + 16 * g;
+            T* const out = static_cast<T*>(a.out) + (static_cast<int64_t>(now.row) * a.heads + head0 + hh) * 128 + 16 * g;
             uint32_t w[8];
 #pragma unroll
             for (int d = 0; d < 8; ++d) w[d] = pack2<T>(o[t][d][i] * inv, o[t][d][2 + i] * inv);
             *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
             *reinterpret_cast<uint4*>(out + 8) = make_uint4(w[4], w[5], w[6], w[7]);
             if (g == 0)
-              a.lse[now.row * a.heads + head0 + hh] =
+              a.lse[static_cast<int64_t>(now.row) * a.heads + head0 + hh] =
                   sum > 0.0f ? (m[t][i] + log2f(sum)) * kLn2 : (sum == 0.0f ? -CUDART_INF_F : sum);
           } else {
             float* const part = a.part + (slot_of_part * kHeads + hh) * 128 + 16 * g;
@@ -714,7 +721,7 @@ Plan plan_for(int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_pages
   Plan p;
   const int64_t per = heads / kv_heads;
   // one 8-column operand where it holds all the heads, else two (64 rows of 1-16 K
-  // tokens: 8 heads a K/V head 110 us with one, 169 with two; 16 heads 184 and 174)
+  // tokens: 8 heads a K/V head 103 us with one, 169 with two; 16 heads 184 and 159)
   p.tiles = per <= 8 ? 1 : 2;
   p.groups = (per + 8 * p.tiles - 1) / (8 * p.tiles);
   p.segments = kv_heads * p.groups;
@@ -735,7 +742,7 @@ void launch_attend(const CUtensorMap& k_map, const CUtensorMap& v_map, const Att
   if (a.ranges == 1) return;
   const unsigned cuts = static_cast<unsigned>(a.ranges - 1), heads = 8 * kTiles;
   // many parts a segment: one row of 4097 tokens 13 us so, 37 with one warp a head; few:
-  // 64 rows of 1-16 K tokens 125 us so, 110 with one
+  // 64 rows of 1-16 K tokens 15 us more than with one
   if (a.ranges >= 16 * a.rows * a.segments)
     launch_join(kv8_join_kernel<T, kTiles, 16>, dim3(static_cast<unsigned>(a.rows * a.segments), heads), dim3(512), s, a);
   else
@@ -826,6 +833,8 @@ extern "C" int v1x_kv8_attend(const void* q, int64_t qs0, int64_t qs1, const uin
                     ((k_cache && k_scale && v_cache && v_scale) || pages == 0),
                 "kv8_attend: NULL argument");
   V1X_CHECK_ARG(pages * kv_heads < (int64_t(1) << 25), "kv8_attend: at most 2^25 pages x K/V heads");
+  V1X_CHECK_ARG(table_pages < (int64_t(1) << 25) && kv_heads * table_pages <= (int64_t(1) << 34) / rows,
+                "kv8_attend: at most 2^25 table columns, 2^34 rows x K/V heads x columns");
   const int64_t need = v1x_kv8_attend_workspace(rows, heads, kv_heads, table_pages);
   V1X_CHECK_ARG(workspace_bytes >= need && (workspace || need == 0) && aligned16(workspace),
                 "kv8_attend: the workspace must be 16-byte aligned and hold %lld bytes", static_cast<long long>(need));

@@ -689,8 +689,8 @@ V1X_API int v1x_kv8_store(uint8_t* k_cache, float* k_scale, uint8_t* v_cache, fl
 /* Softmax attention of q [rows, heads, 128] over the first min(lens[r], 64 *
  * table_pages) tokens of row r in that cache, heads / kv_heads query heads per K/V
  * head; out [rows, heads, 128] in q's type and lse [rows, heads] contiguous.  A page
- * outside the cache holds no tokens.  pages * kv_heads < 2^25.  workspace and status as
- * in v1x_latent_attention. */
+ * outside the cache holds no tokens.  pages * kv_heads < 2^25, table_pages < 2^25, rows *
+ * kv_heads * table_pages <= 2^34.  workspace and status as in v1x_latent_attention. */
 V1X_API int64_t v1x_kv8_attend_workspace(int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_pages);
 V1X_API int v1x_kv8_attend(const void* q, int64_t qs0, int64_t qs1, const uint8_t* k_cache, const float* k_scale,
                   const uint8_t* v_cache, const float* v_scale, int64_t pages, int64_t kv_heads,
