@@ -5,10 +5,22 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace v1x {
 namespace attn {
+
+// Weights that go into a product in f16, whose range ends at 2^16 above and, with steps
+// of 2^-24, at 2^-25 below: taken against a reference 2^lift below the running maximum
+// they use that range up, and many small ones beside a large one are not lost (without
+// it 65536 tokens 17.5 below the largest score lost their 1.6e-3 of the sum).  `lazy`:
+// how far, in powers of two, weights may outgrow their reference.
+template <typename T>
+constexpr float lift(float lazy) {
+  return std::is_same<T, __half>::value ? 15.0f - lazy : 0.0f;
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

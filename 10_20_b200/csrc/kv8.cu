@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(128) kv8_store_kernel(const __grid_constant__ 
 // 64 rows of 1-16 K tokens, 32 heads over 4: 103 us, 5.5 TB/s (the join about 8 of them);
 // one row of 4097 tokens 13 us.
 //   * the query is held in f16 under a power of two per head that puts its largest
-//     value in [1, 2); the weights are rounded to f16 once, sums stay in 32 bits; a
+//     value in [1, 2); the weights, up to 2^15, are rounded to f16 once, sums stay in 32 bits; a
 //     page's output is added under its value scale in 32 bits, so scales of any size
 //     meet the f16 products unchanged.
 struct AttendArgs {
@@ -271,8 +271,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     for (int w = 0; w < kWarps; ++w)
       for (int s = 0; s < kRing; ++s) mbar_init(&sh.full[w][s], 1);
     fence_mbar_init();
-    tma_prefetch_desc(&k_map);
-    tma_prefetch_desc(&v_map);
+    if (a.pages > 0) {
+      tma_prefetch_desc(&k_map);
+      tma_prefetch_desc(&v_map);
+    }
   }
   // ---- this warp's range of the line: pages of row 0's segments, row 1's, ... --------
   const int64_t chunk = (a.rows + kWarps * 32 - 1) / (kWarps * 32);
@@ -493,7 +495,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
             }
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-          top = fmaxf(top, m[t][i]);
+          top = fmaxf(top - lift<__half>(0.0f), m[t][i]);   // m: the weights' reference
           const float ref = top == -CUDART_INF_F ? 0.0f : top;
           alpha[i] = exp2_fast(m[t][i] - ref);
           m[t][i] = top;

@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
 #pragma unroll
       for (int j = 4; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
       float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2)) - lift<T>(kLazy);   // m: the weights' reference
       if (fresh) {
         m = most;
         l = 0.0f;

@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem + quarter + 128 * t, o_addr = tmem + quarter + kOutCol + 128 * t;
     const int mine = t ? n1 : n0;
     const float c = a.scale_log2;
+    constexpr float kLift = lift<T>(kLazy);
     float m = -CUDART_INF_F, l = 0.0f;       // m: of the unscaled scores
     bool ok = true;
     auto wait = [&](uint64_t* bar, int phase) {
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      const float shift = m == -CUDART_INF_F ? 0.0f : -m * c;
+      const float shift = m == -CUDART_INF_F ? 0.0f : kLift - m * c;
       const f32x2 c2 = two(c, c), shift2 = two(shift, shift);
       f32x2 sum[2] = {0, 0};
       uint32_t w[32];
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (i < nq)
-      a.lse[(q0 + i) * a.heads + h] = empty ? -CUDART_INF_F : (m * c + log2f(l)) * kLn2;
+      a.lse[(q0 + i) * a.heads + h] = empty ? -CUDART_INF_F : (m * c - kLift + log2f(l)) * kLn2;
     tc_fence_before();
   } else if (warp < 10) {
     // ---------------- MMA issuers, one per tile ----------------

@@ -51,6 +51,17 @@ def status_word(device: torch.device) -> torch.Tensor:
     return t
 
 
+def status_ptr(device: torch.device) -> int | None:
+    """The status word's address for a call whose waits report into it; None where it is first
+    asked for inside a graph capture, which would record its allocation and zeroing instead."""
+    t = _status.get(device.index)
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        t = status_word(device)
+    return t.data_ptr()
+
+
 def check_status(device=None, reset: bool = True):
     """Raise ArenaExhausted if a kernel on `device` reported an exhausted arena."""
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())

@@ -27,6 +27,7 @@ import torch
 
 from . import _lib
 from ._lib import ptr, require
+from .kernels import status_ptr
 from .latent_attention import PAGE, _DTYPES, _index, _one_device, _outputs, _rows16, _step
 
 
@@ -57,8 +58,8 @@ def store(k_cache, k_scale, v_cache, v_scale, k, v, table, prefix, offsets):
     prefix int32 [requests], offsets int32 [requests + 1] non-decreasing, table
     int32 [requests, pages].  Tokens past the table, or of a page outside the
     cache, are dropped; places of a page behind the last token are left as they
-    are.  No two requests of a call may write the same page.  Storing the same
-    tokens again changes nothing."""
+    are.  A call may write a page for one request and one of its places in the
+    table only.  Storing the same tokens again changes nothing."""
     pages, heads = _cache(k_cache, k_scale, v_cache, v_scale)
     code = _DTYPES.get(k.dtype)
     require(k.dim() == 3 and k.shape[1:] == (heads, 128) and v.shape == k.shape and k.dtype is v.dtype
@@ -108,5 +109,5 @@ def attend(q, k_cache, k_scale, v_cache, v_scale, table, lens, scale, out=None, 
     _lib.call("v1x_kv8_attend", q.data_ptr(), _step(q, 0), _step(q, 1), k_cache.data_ptr(), k_scale.data_ptr(),
               v_cache.data_ptr(), v_scale.data_ptr(), pages, kv_heads, table.data_ptr(), _step(table, 0),
               table.shape[1], lens.data_ptr(), rows, heads, scale, code, out.data_ptr(), lse.data_ptr(), ptr(work), size,
-              None, _lib.stream_of(q), device=device)
+              status_ptr(device), _lib.stream_of(q), device=device)
     return out, lse

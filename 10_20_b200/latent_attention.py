@@ -25,7 +25,9 @@ Every function returns ``(out, lse)``: the attention in q's type and the
 natural logarithm of the sum of exp(s) per row and head (float32).  A row with
 no token has out 0 and lse -inf.  Nothing is synchronised; all work is on the
 current stream of q's device, workspaces come from torch's allocator per call,
-so calls on several streams and captured graphs share nothing.
+so calls on several streams and captured graphs share nothing.  A wait inside a
+kernel that runs out (2 s) is reported in the device's status word, which
+``kernels.check_status`` reads; the call's result is then of no use.
 """
 from __future__ import annotations
 
@@ -36,6 +38,7 @@ import torch
 
 from . import _lib
 from ._lib import ptr, require
+from .kernels import status_ptr
 
 PAGE = 64                                           # tokens per page of the native pool
 _DTYPES = {torch.bfloat16: 1, torch.float16: 2}     # codes shared with v1x_pack_q
@@ -113,7 +116,7 @@ def _absorbed(q, pool, request_slots, index, count, lens, scale, latent, out, ls
     _lib.call("v1x_latent_attention", q.data_ptr(), _step(q, 0), _step(q, 1), pool.data_ptr(), pool.shape[0],
               _step(pool, 0), ptr(request_slots), 0 if request_slots is None else request_slots.shape[0],
               index.data_ptr(), _step(index, 0), count, ptr(lens), rows, heads, dim, latent, scale, code, out.data_ptr(),
-              lse.data_ptr(), ptr(work), size, None, _lib.stream_of(q), device=device)
+              lse.data_ptr(), ptr(work), size, status_ptr(device), _lib.stream_of(q), device=device)
     return out, lse
 
 
@@ -155,7 +158,7 @@ def attend_prompt(q, k, k_rope, v, offsets, scale, kv_offsets=None, out=None, ls
     (bfloat16 / float16), unit inner stride, rows 16-byte aligned -- views of
     one projection's output or of pool rows are taken as they are.  offsets and
     kv_offsets: int32 [requests + 1], non-decreasing, within the tokens.  Rows
-    of q that no request covers are left as they are in out and lse.  A NaN or an
+    of q that no request covers are not written in out and lse.  A NaN or an
     infinity among a request's values also reaches queries that come before it
     (0 times it is NaN); other requests' keys and values are never read."""
     code = _DTYPES.get(q.dtype)
@@ -187,5 +190,5 @@ def attend_prompt(q, k, k_rope, v, offsets, scale, kv_offsets=None, out=None, ls
     _lib.call("v1x_prompt_attention", q.data_ptr(), _step(q, 0), _step(q, 1), k.data_ptr(), _step(k, 0), _step(k, 1),
               ptr(k_rope), 0 if k_rope is None else _step(k_rope, 0), v.data_ptr(), _step(v, 0), _step(v, 1),
               offsets.data_ptr(), kv_offsets.data_ptr(), requests, tokens, keys, heads, dr, scale, code, out.data_ptr(),
-              lse.data_ptr(), None, _lib.stream_of(q), device=device)
+              lse.data_ptr(), status_ptr(device), _lib.stream_of(q), device=device)
     return out, lse

@@ -648,8 +648,8 @@ V1X_API int v1x_gather_slots(const void* k, const void* v, const int32_t* req, c
  * bf16, 2 f16; every address and stride a multiple of 16 bytes.  latent in {128,
  * 256, 384, 512}, dim - latent in {0, 64}, heads <= 1024.  workspace: device
  * memory of at least v1x_latent_attention_workspace(rows, heads, count, latent,
- * lens == NULL) bytes, 16-byte aligned, of no meaning before or after the call (NULL if 0 bytes).  status: optional
- * device word for V1X_STATUS_TIMEOUT. */
+ * lens == NULL) bytes, 16-byte aligned, of no meaning before or after the call
+ * (NULL if 0 bytes).  status: optional device word for V1X_STATUS_TIMEOUT. */
 V1X_API int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, int64_t count, int64_t latent,
                   int equal);
 V1X_API int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, const void* pool, int64_t slots,
@@ -680,7 +680,8 @@ V1X_API int v1x_prompt_attention(const void* q, int64_t qs0, int64_t qs1, const 
  * -40 <= e <= 40, with 448 * 2^e >= the magnitudes stored, and does not fall below
  * the page's former scale if it holds earlier tokens, whose codes are rounded again
  * where it rises.  Tokens past the table or in a page outside the cache are dropped;
- * places behind the last token are not written. */
+ * places behind the last token are not written.  A call may write a page for one
+ * request and one of its places in the table only. */
 V1X_API int v1x_kv8_store(uint8_t* k_cache, float* k_scale, uint8_t* v_cache, float* v_scale, int64_t pages,
                   int64_t heads, const void* k, int64_t ks0, int64_t ks1, const void* v, int64_t vs0, int64_t vs1,
                   int dtype, int64_t tokens, const int32_t* table, int64_t table_stride, int64_t table_pages,

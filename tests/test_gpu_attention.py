@@ -469,6 +469,57 @@ def test_attend_far_scales_pages_and_strides():
     assert not out[2].any() and torch.isinf(lse[2]).all()
 
 
+# -- many small weights beside a few large ones ---------------------------------------
+# Every 64th token scores 17.5, the others 0: weights e^-17.5 = 2^-25.2 of the largest, below what f16 holds (half
+# its smallest step is 2^-25) unless they are lifted into its range.  The large ones' values are 0, so the output
+# consists of the small ones alone.  The floor of a weight, relative to the largest: 2^-25 under the lift, 2^7 in the
+# latent and prompt kernels, 2^15 in the 8-bit ones; their bf16 weights have none.
+def steep(n, dim):
+    k = torch.zeros((n, dim), device=DEV)
+    k[::64, 0] = 4.0
+    v = torch.zeros((n, 128), device=DEV)
+    v[:, 3] = 896.0
+    v[::64, 3] = 0.0
+    q = torch.zeros(dim, device=DEV)
+    q[0] = 4.0
+    return q, k, v, 17.5 / 16
+
+
+def steep_want(q, k, v, scale, dtype, tiny, up):
+    r = dict(u=A.U[dtype], up=up, tiny=tiny, smallest=A.SMALLEST[dtype])
+    return A.softmax_rows(f64(q)[None], f64(k), f64(v), scale, **r)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_small_weights_latent(dtype):
+    q, k, v, scale = steep(2048, 192)
+    k[:, 1:128] = v[:, 1:128]                      # the pool's row is key and value; the query sees its first element
+    floor = 2.0 ** -32 if dtype == "fp16" else 0.0
+    want = [np.broadcast_to(x, (3, 2) + x.shape[1:]) for x in steep_want(q, k, k[:, :128], scale, dtype, floor, A.U[dtype])]
+    t = TYPES[dtype]
+    qs, pool = q.to(t).expand(3, 2, 192).contiguous(), k.to(t)[:, None]
+    check(*L.attend_slots(qs, pool, None, ints(np.arange(2048)[None].repeat(3, 0)), scale, latent=128), want, "slots")
+    check(*L.attend_pages(qs, pool, ints(np.arange(32)[None].repeat(3, 0)), ints([2048] * 3), scale, latent=128), want, "pages")
+    # the third query of three sees every key
+    out, lse = L.attend_prompt(q[:128].to(t).expand(3, 2, 128), k[:, :128].to(t)[:, None].expand(2048, 2, 128), None,
+                               v.to(t)[:, None].expand(2048, 2, 128), ints([0, 3]), scale, kv_offsets=ints([0, 2048]))
+    want = [np.broadcast_to(x, (2,) + x.shape[1:]) for x in steep_want(q[:128], k[:, :128], v, scale, dtype, floor, A.U[dtype])]
+    check(out[2], lse[2], want, "prompt")
+
+
+@pytest.mark.parametrize("dtype,heads", [("bf16", 4), ("fp16", 40)])
+def test_small_weights_8bit(dtype, heads):
+    q, k, v, scale = steep(2048, 128)
+    c = new_cache(32, 1)
+    t = TYPES[dtype]
+    # exact: 4 and 896 are codes under their pages' scales
+    K.store(*c, k.to(t)[:, None], v.to(t)[:, None], ints(np.arange(32)[None]), ints([0]), ints([0, 2048]))
+    out, lse = K.attend(q.to(t).expand(1, heads, 128).contiguous(), *c, ints(np.arange(32)[None]), ints([2048]), scale)
+    want = [np.broadcast_to(x, (1, heads) + x.shape[1:])
+            for x in steep_want(q, k, v, scale, dtype, 2.0 ** -40, 2.0 ** -11)]
+    check(out, lse, want)
+
+
 # -- streams, graphs, the pieces together ---------------------------------------------
 def calls():
     """Small calls of every operator: name -> (inputs, function of the inputs)."""
@@ -611,7 +662,7 @@ def test_selection_step_attends():
     pipeline = importlib.import_module("10_20_b200.pipeline")
     case = synth.make_query_case(3, 64, [4097, 9000, 700], P=256, take=12, window=64, topk=2048, seed=3, device=DEV,
                                  latent_dim=576)
-    q = normal((3, 16, 576), "bf16", 93)
+    q = normal((3, 24, 576), "bf16", 93)
     step = pipeline.SelectionStep(case, gather=False, attention=(q, 0.07))
     step.run()
     torch.cuda.synchronize()
@@ -620,7 +671,7 @@ def test_selection_step_attends():
     check(*step.attended, want_slots(q, case.latent, step.physical, 0.07, 512, "bf16"))
     step.capture()
     step.attended[0].zero_()
-    q.copy_(normal((3, 16, 576), "bf16", 94))
+    q.copy_(normal((3, 24, 576), "bf16", 94))
     step.replay()
     want = L.attend_slots(q, case.latent, None, step.physical, 0.07)
     assert torch.equal(step.attended[0], want[0]) and torch.equal(step.attended[1], want[1])
