@@ -7,6 +7,8 @@ Drop-in modules mirroring the reference's operator surfaces:
   fused_grouping  _sort                            (v1_native/fused_grouping.py)
   gather          _gather_slots, GatherWorkspace   (v1_native/kernels.py)
   scoring         fp8_paged_mqa_logits             (DeepGEMM contract)
+  latent_attention  attend_slots, attend_pages, attend_prompt: absorbed and expanded latent attention
+  kv8               store, attend: the paged 8-bit K/V cache and its decode
 and the composed step (`pipeline.SelectionStep`) plus seeded synthetic
 workloads (`synth`).  All compute runs in libv1x.so; there is no CPU path.
 
