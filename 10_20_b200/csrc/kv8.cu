@@ -1,6 +1,5 @@
 // The paged 8-bit K/V cache: v1x_kv8_store and v1x_kv8_attend of v1x.h.
 #include <cuda_fp8.h>
-#include <cudaTypedefs.h>
 
 #include <type_traits>
 
@@ -753,14 +752,7 @@ void launch_attend(const CUtensorMap& k_map, const CUtensorMap& v_map, const Att
 
 // Rows of 128 codes, 64 (a page and head) a box, 128-byte swizzle.
 int encode_cache(CUtensorMap* map, const uint8_t* cache, int64_t blocks) {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  }();
+  const PFN_cuTensorMapEncodeTiled_v12000 fn = map_encoder();
   if (!fn) {
     set_error("kv8_attend: cuTensorMapEncodeTiled unavailable");
     return V1X_ERR_CUDA;

@@ -22,7 +22,7 @@
 // (load 2000 cycles, scores 1500, softmax 1400, output 600; 3600 a tile with two in
 // flight, of which its MMAs need 1920).  So a tile is loaded, weighted and released
 // in two halves of 32 tokens, and its scores begin on the first blocks.  128 rows of
-// 2048 tokens, 64 heads: 81 us, 3.9 TB/s; 1024 rows, 128 heads: 953 us, 613 TFLOP/s.
+// 2048 tokens, 64 heads: 81 us, 3.9 TB/s; 1024 rows, 128 heads: 929 us, 628 TFLOP/s.
 // Measured and not kept: four tiles of 32 (80 and 1004 us: N = 32 costs the scores a
 // quarter of the rate), whole pages by TMA (116 instead of 107 us on 48 ragged rows),
 // each half copied by all eight warps in turn (103 us); the tensor-map gather of four
@@ -83,7 +83,7 @@ struct LatentArgs {
   float scale_log2;
   void* out;
   float* lse;
-  float* part;       // [ranges * groups][2][64][latent], then [..][2][64][2] maxima and sums
+  float* part;       // [ranges * groups][2][16][latent][4]: four heads' values side by side; then [..][2][2][64] maxima, sums
   float* part_ml;
   int64_t* where;    // [ranges + 1][4]: where range x begins: the row, its first tile in the line, its
                      // tiles, and the range's own first tile; [ranges][3]: the number of all tiles
@@ -414,8 +414,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
             sh.factor[h] = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
             if (h < heads) a.lse[o] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
           } else if (h < heads) {
-            a.part_ml[(slot * kGroup + h) * 2] = m;
-            a.part_ml[(slot * kGroup + h) * 2 + 1] = l;
+            a.part_ml[slot * 2 * kGroup + h] = m;
+            a.part_ml[slot * 2 * kGroup + kGroup + h] = l;
           }
         }
         sync_128();
@@ -462,10 +462,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
               uint32_t o[32];
               tmem_ld32(tmem + quarter + t * 64 + c, o);
               tmem_ld_wait();
-              float* const to = part + c * kLatent + t * 128 + d;
+              float* const to = part + c * kLatent + (t * 128 + d) * 4;
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (c + j < heads) to[j * kLatent] = __uint_as_float(o[j]);
+              for (int j = 0; j < 32; j += 4)
+                if (c + j < heads)
+                  *reinterpret_cast<float4*>(to + j * kLatent) =
+                      make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
             }
         }
         tc_fence_before();
@@ -645,88 +647,111 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
 
 // Joins the parts of the rows that lie in several ranges, in the order of the
 // ranges.  Range y's part is its first (slot 0) unless the range begins in an
-// earlier row (then its last, slot 1); a range may be empty.
-//   kWarps = 1: a warp joins one head's whole row (grid y: four heads) -- two or
-//     three parts each, many rows.  Grid x: the row in which range x + 1 begins, if
-//     that is the first range to begin inside it;
-//   kWarps = 4: the four warps of a block share the parts of one head and 128
-//     of its columns (grid z) -- a few rows (grid x) spread over all ranges.
-// Measured, both kernels together: one row of 131072 tokens 125 us with one warp, 62
-// with four; 48 ragged rows of 1-16384 tokens 106.7 and 107.4.
-template <typename T, int kLatent, int kWarps>
-__global__ void __launch_bounds__(128) latent_join_kernel(const __grid_constant__ LatentArgs a) {
-  constexpr int kPer = kWarps == 1 ? kLatent / 128 : 1;   // 16-byte pieces of a lane
+// earlier row (then its last, slot 1); a range may be empty.  A warp has four heads
+// (grid y) and 64 columns at a time, a lane two of them: 32 bytes of a part.
+//   kShare = 1: a warp joins all parts -- two or three, many rows; the block's warps
+//     have all columns.  Grid x: the row in which range x + 1 begins, if that
+//     is the first range to begin inside it;
+//   kShare = 16: the block's warps share the parts of 64 columns (grid z) -- a few
+//     rows (grid x) spread over all ranges.
+// One row of 131072 tokens: both kernels 53.5 us; with a warp for each head and four
+// warps to share its parts 62, with one 125.
+template <typename T, int kLatent, int kShare>
+__global__ void __launch_bounds__(kShare == 1 ? kLatent / 2 : 32 * kShare) latent_join_kernel(const __grid_constant__ LatentArgs a) {
   wait_for_previous();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = kWarps == 1 ? static_cast<int>(blockIdx.y) * 4 + warp : static_cast<int>(blockIdx.y);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = 4 * blockIdx.y;
   int x = blockIdx.x + 1;
-  if constexpr (kWarps == 4) {
+  if constexpr (kShare > 1) {
     __shared__ int found;
     if (threadIdx.x == 0) found = kMaxCtas;
     __syncthreads();
-    for (int i = threadIdx.x + 1; i < a.ranges; i += 128)
+    for (int i = threadIdx.x + 1; i < a.ranges; i += 32 * kShare)
       if (a.where[4 * i] == blockIdx.x && a.where[4 * i + 3] > a.where[4 * i + 1]) atomicMin(&found, i);
     __syncthreads();
     x = found;
     if (x == kMaxCtas) return;
   }
   const int64_t first = a.where[4 * x + 1], begin = a.where[4 * x + 3], before = a.where[4 * x - 1];
-  if (begin == first || before > first || h >= a.heads) return;   // kWarps = 4: the whole block
+  if (begin == first || before > first) return;              // the whole block
   const int64_t row = a.where[4 * x], end = first + a.where[4 * x + 2];
-  const int64_t step = static_cast<int64_t>(a.groups) * 2 * kGroup;
-  const int64_t base = (static_cast<int64_t>(x - 1) * a.groups + h / kGroup) * 2 * kGroup + h % kGroup;
-  const int64_t shift = before < first ? kGroup : 0;   // range x - 1 may begin in an earlier row
-  auto part = [&](int i) { return base + i * step + (i == 0 ? shift : 0); };
-  float m = -CUDART_INF_F, l = 0.0f;
+  // the part of range x - 1 + i, which may begin in an earlier row if i is 0
+  const int64_t base = (static_cast<int64_t>(x - 1) * a.groups + h / kGroup) * 2, step = 2 * a.groups;
+  auto part = [&](int i) { return base + i * step + (i == 0 && before < first ? 1 : 0); };
+  auto live = [&](int i) { return a.where[4 * (x + i) + 3] > a.where[4 * (x - 1 + i) + 3]; };
+  auto four = [](const float* p) { return *reinterpret_cast<const float4*>(p); };
+  const float* const ml = a.part_ml + h % kGroup;
+  float4 m = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
   int parts = 0;
   for (int i = lane; i <= a.ranges - x; i += 32) {
-    const int64_t t0 = a.where[4 * (x - 1 + i) + 3], t1 = a.where[4 * (x + i) + 3];
-    if (t0 >= end) break;
+    if (a.where[4 * (x - 1 + i) + 3] >= end) break;
     parts = i + 1;
-    if (t1 > t0) m = fmaxf(m, a.part_ml[2 * part(i)]);
+    if (!live(i)) continue;
+    const float4 v = four(ml + part(i) * 2 * kGroup);
+    m = make_float4(fmaxf(m.x, v.x), fmaxf(m.y, v.y), fmaxf(m.z, v.z), fmaxf(m.w, v.w));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m.x = fmaxf(m.x, __shfl_xor_sync(0xffffffffu, m.x, o));
+    m.y = fmaxf(m.y, __shfl_xor_sync(0xffffffffu, m.y, o));
+    m.z = fmaxf(m.z, __shfl_xor_sync(0xffffffffu, m.z, o));
+    m.w = fmaxf(m.w, __shfl_xor_sync(0xffffffffu, m.w, o));
     parts = max(parts, __shfl_xor_sync(0xffffffffu, parts, o));
   }
-  const float ref = m == -CUDART_INF_F ? 0.0f : m;
-  float4 o[kPer];
-#pragma unroll
-  for (int c = 0; c < kPer; ++c) o[c] = make_float4(0, 0, 0, 0);
-  const int column = kWarps == 1 ? 4 * lane : static_cast<int>(blockIdx.z) * 128 + 4 * lane;
-#pragma unroll(kWarps == 1 ? 2 : 8)
-  for (int i = kWarps == 1 ? 0 : warp; i < parts; i += kWarps) {
-    if (a.where[4 * (x + i) + 3] == a.where[4 * (x - 1 + i) + 3]) continue;
-    const float w = exp2f(a.part_ml[2 * part(i)] - ref);
-    l += a.part_ml[2 * part(i) + 1] * w;
-#pragma unroll
-    for (int c = 0; c < kPer; ++c) {
-      const float4 v = *reinterpret_cast<const float4*>(a.part + part(i) * kLatent + column + 128 * c);
-      o[c] = make_float4(fmaf(v.x, w, o[c].x), fmaf(v.y, w, o[c].y), fmaf(v.z, w, o[c].z), fmaf(v.w, w, o[c].w));
-    }
+  auto ref = [](float v) { return v == -CUDART_INF_F ? 0.0f : v; };
+  const float4 r = make_float4(ref(m.x), ref(m.y), ref(m.z), ref(m.w));
+  auto add = [](float4& o, const float4& v, const float4& w) {
+    o = make_float4(fmaf(v.x, w.x, o.x), fmaf(v.y, w.y, o.y), fmaf(v.z, w.z, o.z), fmaf(v.w, w.w, o.w));
+  };
+  auto inverse = [](float l) { return l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l); };
+  auto lse_of = [](float m_, float l) { return l > 0.0f ? (m_ + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l); };
+  T* const out = static_cast<T*>(a.out) + (row * a.heads + h) * kLatent;
+  const int heads = min(4, static_cast<int>(a.heads - h));
+  const int block = kShare == 1 ? warp : static_cast<int>(blockIdx.z);
+  const float4 none = make_float4(0, 0, 0, 0);
+  float4 l = none, o0 = none, o1 = none;       // o0, o1: of columns 64 block + 2 lane, + 1
+  const float* const from = a.part + static_cast<int64_t>(h % kGroup) * kLatent + (64 * block + 2 * lane) * 4;
+#pragma unroll(kShare == 1 ? 2 : 5)
+  for (int i = kShare == 1 ? 0 : warp; i < parts; i += kShare) {
+    const bool some = live(i);               // the slot of an empty range holds nothing
+    const float* const p = from + part(i) * kGroup * kLatent;
+    const float4 v0 = some ? four(p) : none, v1 = some ? four(p + 4) : none;
+    const float4 lp = some ? four(ml + part(i) * 2 * kGroup + kGroup) : none;
+    const float4 mp = some ? four(ml + part(i) * 2 * kGroup) : r;
+    const float4 w = make_float4(exp2f(mp.x - r.x), exp2f(mp.y - r.y), exp2f(mp.z - r.z), exp2f(mp.w - r.w));
+    add(l, lp, w);
+    add(o0, v0, w);
+    add(o1, v1, w);
   }
-  if constexpr (kWarps == 4) {
-    __shared__ float4 sums[4][32];
-    __shared__ float ls[4];
-    sums[warp][lane] = o[0];
+  if constexpr (kShare > 1) {
+    __shared__ float4 sums[kShare][64], ls[kShare];
+    sums[warp][2 * lane] = o0;
+    sums[warp][2 * lane + 1] = o1;
     if (lane == 0) ls[warp] = l;
     __syncthreads();
-    if (warp > 0) return;
-    l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
-    for (int w = 1; w < 4; ++w) {
-      const float4 v = sums[w][lane];
-      o[0] = make_float4(o[0].x + v.x, o[0].y + v.y, o[0].z + v.z, o[0].w + v.w);
+    const int column = threadIdx.x & 63, k = threadIdx.x >> 6;   // one head's column a thread
+    if (k >= heads) return;
+    float o = 0.0f, all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kShare; ++w) {
+      o += reinterpret_cast<const float*>(&sums[w][column])[k];
+      all += reinterpret_cast<const float*>(&ls[w])[k];
+    }
+    reinterpret_cast<uint16_t*>(out)[k * kLatent + 64 * block + column] = static_cast<uint16_t>(pack2<T>(o * inverse(all), 0.0f));
+    if (block == 0 && column == 0) {
+      const float top = k == 0 ? m.x : k == 1 ? m.y : k == 2 ? m.z : m.w;
+      a.lse[row * a.heads + h + k] = lse_of(top, all);
+    }
+  } else {
+    const float os[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w}, lk[4] = {l.x, l.y, l.z, l.w};
+    const float mk[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k >= heads) break;
+      const float inv = inverse(lk[k]);
+      *reinterpret_cast<uint32_t*>(out + k * kLatent + 64 * block + 2 * lane) = pack2<T>(os[k] * inv, os[4 + k] * inv);
+      if (block == 0 && lane == 0) a.lse[row * a.heads + h + k] = lse_of(mk[k], lk[k]);
     }
   }
-  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-  T* const out = static_cast<T*>(a.out) + (row * a.heads + h) * kLatent + column;
-#pragma unroll
-  for (int c = 0; c < kPer; ++c)
-    *reinterpret_cast<uint2*>(out + 128 * c) =
-        make_uint2(pack2<T>(o[c].x * inv, o[c].y * inv), pack2<T>(o[c].z * inv, o[c].w * inv));
-  if (lane == 0 && column == 0)
-    a.lse[row * a.heads + h] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
 }
 
 constexpr int64_t kMaxSmem = 232448;
@@ -771,11 +796,11 @@ void launch(LatentArgs a, bool join, cudaStream_t s) {
   launch_kernel_prio(LaunchPriority::kDefault, latent_kernel<T, kLatent, kRope>,
                      dim3(static_cast<unsigned>(a.ranges * a.groups)), dim3(kThreads), kSmem, s, a);
   if (!join) return;
-  const unsigned cuts = static_cast<unsigned>(a.ranges - 1), heads = static_cast<unsigned>(a.heads);
+  const unsigned cuts = static_cast<unsigned>(a.ranges - 1), fours = static_cast<unsigned>((a.heads + 3) / 4);
   if (a.ranges >= 8 * a.rows)
-    launch_join(latent_join_kernel<T, kLatent, 4>, dim3(static_cast<unsigned>(a.rows), heads, kLatent / 128), dim3(128), s, a);
+    launch_join(latent_join_kernel<T, kLatent, 16>, dim3(static_cast<unsigned>(a.rows), fours, kLatent / 64), dim3(512), s, a);
   else
-    launch_join(latent_join_kernel<T, kLatent, 1>, dim3(cuts, (heads + 3) / 4), dim3(128), s, a);
+    launch_join(latent_join_kernel<T, kLatent, 1>, dim3(cuts, fours), dim3(kLatent / 2), s, a);
 }
 
 template <typename T>

@@ -36,8 +36,6 @@
 // then keys and values.  Later queries see more keys: the grid begins with the last
 // ones, all heads of a tile side by side.
 // Waits are bounded (2 s, then V1X_STATUS_TIMEOUT).
-#include <cudaTypedefs.h>
-
 #include <type_traits>
 
 #include "attention.cuh"
@@ -457,14 +455,7 @@ static_assert(kSmem <= 232448, "shared memory");
 // takes no such map.
 bool encode_rows(CUtensorMap* map, bool bf16, const void* p, int64_t keys, int64_t heads, int64_t key_stride,
                  int64_t head_stride) {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  }();
+  const PFN_cuTensorMapEncodeTiled_v12000 fn = map_encoder();
   if (!fn) return false;
   const cuuint32_t steps[3] = {1, 1, 1};
   const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
