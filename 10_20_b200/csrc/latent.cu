@@ -654,8 +654,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
 //     is the first range to begin inside it;
 //   kShare = 16: the block's warps share the parts of 64 columns (grid z) -- a few
 //     rows (grid x) spread over all ranges.
-// One row of 131072 tokens: both kernels 53.5 us; with a warp for each head and four
-// warps to share its parts 62, with one 125.
+// Both kernels: one row of 131072 tokens 111 us with one, 53.5 with sixteen (62 with
+// four and a head a warp); 512 tokens 15.4 and 13.1; 48 ragged rows 107 and 123.
 template <typename T, int kLatent, int kShare>
 __global__ void __launch_bounds__(kShare == 1 ? kLatent / 2 : 32 * kShare) latent_join_kernel(const __grid_constant__ LatentArgs a) {
   wait_for_previous();
@@ -760,8 +760,8 @@ constexpr int64_t kMaxSmem = 232448;
 // first `extra` ones a unit more.  Ranges that cut rows cost their parts' traffic
 // and a second launch, about as long as kJoinTiles tiles of a CTA, so rows of equal
 // length go whole to the CTAs where the longest range is not longer by more than
-// that.  128 rows of 2048 tokens, 64 heads: 81 us whole on 128 CTAs, 88 cut into 148;
-// 1024 rows, 128 heads: 953 and 962.
+// that.  128 rows of 2048 tokens, 64 heads: 81 us whole on 128 CTAs, 92 cut into 148;
+// 1024 rows, 128 heads: 929 and 952.
 struct Cut {
   int64_t ranges, unit, base, extra;
   bool whole;
