@@ -32,7 +32,8 @@
 // the groups of 64 heads, neighbours in the grid, which read the same tiles at the
 // same time from L2).  A row that lies in several ranges leaves unnormalised parts
 // in the workspace, joined by latent_join_kernel in the order of the ranges; rows
-// of equal length are given to the CTAs whole where that is no longer (cut_for).
+// of equal length are given to the CTAs whole where that is no longer, and a few of
+// them to a cluster each, whose CTAs join their parts through shared memory (cut_for).
 //
 // Warp roles (512 threads, one CTA per SM):
 //   0-3   softmax, rescale, epilogue (TMEM lane quarters 0-3)
@@ -46,6 +47,8 @@
 //         the tensor cores idle (111 us instead of 92 on the decode batch)
 //   15    the queries, when the row changes
 // Waits are bounded (2 s, then V1X_STATUS_TIMEOUT).
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 #include "attention.cuh"
@@ -79,6 +82,7 @@ struct LatentArgs {
   const int32_t* lens;
   int64_t rows, heads;
   int pairs, groups, ranges;
+  int share;                   // CTAs of a cluster, which have a row's tiles together
   int64_t unit, base, extra;   // the cut of the line in units of `unit` tiles (lens: unit 1, on the device)
   float scale_log2;
   void* out;
@@ -101,6 +105,7 @@ struct LatentShared {
   uint64_t mask[kMaxPairs];
   uint32_t flags[kMaxPairs];
   alignas(16) float factor[kGroup];
+  float m[kGroup], l[kGroup];      // of a cluster's CTA
   int64_t start[4];  // as LatentArgs::where, but [3]: all tiles
   int64_t cut[2];    // base, extra
   int64_t scan[kThreads / 32 + 1];
@@ -203,7 +208,8 @@ struct RowCopy {
   }
 };
 
-template <typename T, int kLatent, int kRope>
+// kCluster: the CTAs of a cluster have one row, an equal part of its tiles each.
+template <typename T, int kLatent, int kRope, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_constant__ LatentArgs a) {
   constexpr int kChunks = (kLatent + kRope) / 64, kOut = kLatent / 128;
   constexpr int kEarly = (kChunks + 1) / 2;   // the blocks that the scores begin with
@@ -216,8 +222,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   const uint32_t p_smem = smem_u32(p_ptr);
   LatentShared& sh = *reinterpret_cast<LatentShared*>(p_ptr + kBlock);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int group = blockIdx.x % a.groups;
-  const int64_t x = blockIdx.x / a.groups;
+  const int rank = kCluster ? blockIdx.x % a.share : 0, cta = kCluster ? blockIdx.x / a.share : blockIdx.x;
+  const int group = cta % a.groups;
+  const int64_t x = cta / a.groups;            // the range; kCluster: the row
   const int heads = min(kGroup, static_cast<int>(a.heads - group * kGroup));
 
   if (tid == 0) {
@@ -246,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   if (!a.lens) {
     if (tid == 0) {
       const int64_t per = (a.count + kTile - 1) / kTile, t0 = range_start(x, a.unit, a.base, a.extra);
-      const int64_t row = per ? (t0 >> 31 ? t0 / per : static_cast<uint32_t>(t0) / static_cast<uint32_t>(per)) : 0;
+      const int64_t row = kCluster ? x : per ? (t0 >> 31 ? t0 / per : static_cast<uint32_t>(t0) / static_cast<uint32_t>(per)) : 0;
       sh.start[0] = row;
       sh.start[1] = row * per;
       sh.start[2] = per;
@@ -286,8 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   }
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  const int64_t t0 = range_start(x, a.unit, sh.cut[0], sh.cut[1]);
-  const int n = static_cast<int>(range_start(x + 1, a.unit, sh.cut[0], sh.cut[1]) - t0);   // tiles of the range
+  const int64_t per = sh.start[2];
+  const int64_t t0 = kCluster ? x * per + per * rank / a.share : range_start(x, a.unit, sh.cut[0], sh.cut[1]);
+  const int64_t t1 = kCluster ? x * per + per * (rank + 1) / a.share : range_start(x + 1, a.unit, sh.cut[0], sh.cut[1]);
+  const int n = static_cast<int>(t1 - t0);     // tiles of the range
   Place at{static_cast<int>(sh.start[0]), static_cast<int>(t0 - sh.start[1]), static_cast<int>(sh.start[2])};
   if (tid == 0 && group == 0 && a.where) {
     for (int i = 0; i < 3; ++i) a.where[4 * x + i] = sh.start[i];
@@ -405,6 +414,28 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
         wait(&sh.pv_done[1], it);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         tc_fence_after();
+        if constexpr (kCluster) {
+          // the CTA's only segment: its part goes where queries and tiles were, 64 columns of
+          // all heads side by side
+          if (mine) {
+            sh.m[h] = m;
+            sh.l[h] = l;
+          }
+#pragma unroll 1
+          for (int t = 0; t < kOut; ++t)
+#pragma unroll 1
+            for (int c = 0; c < cols; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(tmem + quarter + t * 64 + c, o);
+              tmem_ld_wait();
+              float* const to = reinterpret_cast<float*>(base) + ((2 * t + (warp >> 1)) * kGroup + c) * 64 + (warp & 1) * 32 + lane;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (c + j < heads) to[j * 64] = __uint_as_float(o[j]);
+            }
+          tc_fence_before();
+          break;
+        }
         const bool whole = at.last() && segment_tile == 0;   // all of the row's tiles were here
         const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (segment > 0 ? 1 : 0));
         float* part = a.part + slot * kGroup * kLatent;
@@ -643,6 +674,46 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if constexpr (kCluster) {
+    // ---- a CTA joins every share-th 64 columns of the cluster's parts ----------------
+    auto cluster = cooperative_groups::this_cluster();
+    float* const weight = reinterpret_cast<float*>(p_ptr), * const sum = weight + 8 * kGroup;   // [share][64]
+    cluster.sync();                            // all parts are there
+    for (int i = tid; i < a.share * kGroup; i += kThreads) {
+      weight[i] = *cluster.map_shared_rank(&sh.m[i % kGroup], i / kGroup);
+      sum[i] = *cluster.map_shared_rank(&sh.l[i % kGroup], i / kGroup);
+    }
+    __syncthreads();
+    if (tid < heads) {
+      float m = -CUDART_INF_F, l = 0.0f;
+      for (int p = 0; p < a.share; ++p) m = fmaxf(m, weight[p * kGroup + tid]);
+      const float ref = m == -CUDART_INF_F ? 0.0f : m;
+      for (int p = 0; p < a.share; ++p) l += sum[p * kGroup + tid] * exp2f(weight[p * kGroup + tid] - ref);
+      const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+      for (int p = 0; p < a.share; ++p) weight[p * kGroup + tid] = exp2f(weight[p * kGroup + tid] - ref) * inv;
+      if (rank == 0)
+        a.lse[x * a.heads + group * kGroup + tid] = l > 0.0f ? (m + log2f(l)) * kLn2 : (l == 0.0f ? -CUDART_INF_F : l);
+    }
+    __syncthreads();
+    T* const out = static_cast<T*>(a.out) + (x * a.heads + group * kGroup) * kLatent;
+    for (int block = rank; block < kLatent / 64; block += a.share)
+      for (int i = tid; i < heads * 16; i += kThreads) {
+        const int h = i >> 4, column = 4 * (i & 15);
+        float4* const from = reinterpret_cast<float4*>(base) + (block * kGroup + h) * 16 + (i & 15);
+        float4 o = make_float4(0, 0, 0, 0), v[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+          if (p < a.share) v[p] = *cluster.map_shared_rank(from, p);
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+          if (p < a.share) {
+            const float w = weight[p * kGroup + h];
+            o = make_float4(fmaf(v[p].x, w, o.x), fmaf(v[p].y, w, o.y), fmaf(v[p].z, w, o.z), fmaf(v[p].w, w, o.w));
+          }
+        *reinterpret_cast<uint2*>(out + h * kLatent + 64 * block + column) = make_uint2(pack2<T>(o.x, o.y), pack2<T>(o.z, o.w));
+      }
+    cluster.sync();                            // read by all before it goes
+  }
 }
 
 // Joins the parts of the rows that lie in several ranges, in the order of the
@@ -655,7 +726,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
 //   kShare = 16: the block's warps share the parts of 64 columns (grid z) -- a few
 //     rows (grid x) spread over all ranges.
 // Both kernels: one row of 131072 tokens 111 us with one, 53.5 with sixteen (62 with
-// four and a head a warp); 512 tokens 15.4 and 13.1; 48 ragged rows 107 and 123.
+// four and a head a warp); 512 tokens 15.4 and 13.1; 12 rows of 2048 30 and 38; 48
+// ragged rows 107 and 123.
 template <typename T, int kLatent, int kShare>
 __global__ void __launch_bounds__(kShare == 1 ? kLatent / 2 : 32 * kShare) latent_join_kernel(const __grid_constant__ LatentArgs a) {
   wait_for_previous();
@@ -762,22 +834,51 @@ constexpr int64_t kMaxSmem = 232448;
 // length go whole to the CTAs where the longest range is not longer by more than
 // that.  128 rows of 2048 tokens, 64 heads: 81 us whole on 128 CTAs, 92 cut into 148;
 // 1024 rows, 128 heads: 929 and 952.
+// A few rows go to a cluster of 2, 4 or 8 CTAs each, which needs no second kernel but
+// costs about kClusterTiles more than the first, while the second takes a tile's time
+// for each row and group of heads up to kJoinMost.  2048 tokens, 64 heads, clusters and
+// cut: 4 rows 21.5 and 21.2 us, 8 rows 21.1 and 29.4, 14 rows 23.2 and 29.8, 32 rows 33.5
+// and 39.1, 64 rows 48.9 and 57.3; one row of 512 tokens 15.1 and 13.1.  15 clusters of
+// 8 were resident at once, 16 were not (42.8 us).
 struct Cut {
-  int64_t ranges, unit, base, extra;
+  int64_t ranges, unit, base, extra, share;
   bool whole;
 };
-constexpr int64_t kJoinTiles = 6;
+constexpr int64_t kJoinTiles = 6, kClusterTiles = 1, kJoinMost = 5;
 
 Cut cut_for(int64_t rows, int64_t heads, int64_t count, bool equal) {
-  const int64_t fit = kMaxCtas / ((heads + kGroup - 1) / kGroup), per = (count + kTile - 1) / kTile;
+  const int64_t groups = (heads + kGroup - 1) / kGroup, fit = kMaxCtas / groups, per = (count + kTile - 1) / kTile;
   const int64_t tiles = rows * per, ranges = tiles < fit ? (tiles > 0 ? tiles : 1) : fit;
-  Cut c{ranges, 1, tiles / ranges, tiles % ranges, false};
+  Cut c{ranges, 1, tiles / ranges, tiles % ranges, 1, false};
   const int64_t turns = (rows + fit - 1) / fit;
   if (equal && (ranges == 1 || turns * per <= (tiles + ranges - 1) / ranges + kJoinTiles)) {
     c.ranges = (rows + turns - 1) / turns;
-    c = Cut{c.ranges, per, rows / c.ranges, rows % c.ranges, true};
+    c = Cut{c.ranges, per, rows / c.ranges, rows % c.ranges, 1, true};
+  }
+  if (equal) {
+    int64_t share = 8;
+    while (share > 1 && (share > per || rows * groups * share > (share == 8 ? 112 : 128))) share /= 2;
+    const int64_t join = rows * groups - 1 < kJoinMost ? rows * groups - 1 : kJoinMost;
+    const int64_t each = (per + share - 1) / share, now = c.whole ? turns * per : (tiles + ranges - 1) / ranges + join;
+    if (share > 1 && each + kClusterTiles <= now) c = Cut{rows, 1, per, 0, share, true};
   }
   return c;
+}
+
+template <typename... KArgs>
+void launch_clusters(void (*kernel)(KArgs...), int64_t clusters, int share, size_t smem, cudaStream_t s, KArgs... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * share));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = share;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // Launches the kernels of one element type and one pair of widths.
@@ -791,13 +892,16 @@ void launch(LatentArgs a, bool join, cudaStream_t s) {
   a.pairs = kPairs;
   static DeviceOnce once;
   once.run([] {
-    cudaFuncSetAttribute(latent_kernel<T, kLatent, kRope>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    cudaFuncSetAttribute(latent_kernel<T, kLatent, kRope, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    cudaFuncSetAttribute(latent_kernel<T, kLatent, kRope, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
-  launch_kernel_prio(LaunchPriority::kDefault, latent_kernel<T, kLatent, kRope>,
+  if (a.share > 1)
+    return launch_clusters(latent_kernel<T, kLatent, kRope, true>, a.rows * a.groups, a.share, kSmem, s, a);
+  launch_kernel_prio(LaunchPriority::kDefault, latent_kernel<T, kLatent, kRope, false>,
                      dim3(static_cast<unsigned>(a.ranges * a.groups)), dim3(kThreads), kSmem, s, a);
   if (!join) return;
   const unsigned cuts = static_cast<unsigned>(a.ranges - 1), fours = static_cast<unsigned>((a.heads + 3) / 4);
-  if (a.ranges >= 8 * a.rows)
+  if (a.ranges >= 8 * a.rows && a.rows * a.heads <= 512)
     launch_join(latent_join_kernel<T, kLatent, 16>, dim3(static_cast<unsigned>(a.rows), fours, kLatent / 64), dim3(512), s, a);
   else
     launch_join(latent_join_kernel<T, kLatent, 1>, dim3(cuts, fours), dim3(kLatent / 2), s, a);
@@ -851,7 +955,7 @@ extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, con
   const int64_t groups = (heads + kGroup - 1) / kGroup;
   const Cut c = cut_for(rows, heads, count, lens == nullptr);
   LatentArgs a{q,    qs0,  qs1,   pool, slots, pool_stride, req, req_len, index, index_stride, count, lens, rows, heads,
-               0, static_cast<int>(groups), static_cast<int>(c.ranges), c.unit, c.base, c.extra, scale * kLog2e, out,
+               0, static_cast<int>(groups), static_cast<int>(c.ranges), static_cast<int>(c.share), c.unit, c.base, c.extra, scale * kLog2e, out,
                lse, nullptr, nullptr, nullptr, status};
   if (need) {
     a.where = static_cast<int64_t*>(workspace);

@@ -95,6 +95,30 @@ def test_slots_scales(scale):
     check(*L.attend_slots(q, pool, None, ids, scale), want_slots(q, pool, ids, scale, 512, "bf16"))
 
 
+@pytest.mark.parametrize("rows,heads,top,latent,rope,dtype", [
+    (8, 64, 2048, 512, 64, "bf16"), (10, 3, 640, 128, 0, "fp16"), (30, 70, 300, 256, 64, "bf16"), (14, 33, 575, 384, 64, "fp16"),
+    (24, 64, 520, 512, 0, "bf16"), (60, 9, 321, 512, 64, "fp16"), (7, 130, 1000, 128, 64, "bf16"),
+])
+def test_slots_rows_of_clusters(rows, heads, top, latent, rope, dtype):
+    """A few rows, whose CTAs join through shared memory (no workspace): parts of unequal size, a row without a
+    token, rows whose tokens are all in one part, a part whose scores dwarf the others'."""
+    assert L.workspace_bytes(rows, heads, top, latent, True) == 0
+    q, pool = normal((rows, heads, latent + rope), dtype, 101), normal((3000, 1, latent + rope), dtype, 102)
+    pool[17] *= 8
+    ids = np.random.default_rng(103).integers(0, 3000, (rows, top))
+    ids[0] = -1
+    ids[1, :top - 1] = -1
+    ids[2, 1:] = -1
+    ids[3, top // 2] = 17
+    ids[4, ::2] = 3000
+    ids = ints(ids)
+    out, lse = L.attend_slots(q, pool, None, ids, 0.06, latent=latent)
+    check(out, lse, want_slots(q, pool, ids, 0.06, latent, dtype))
+    assert not out[0].any() and torch.isinf(lse[0]).all()
+    again = L.attend_slots(q, pool, None, ids, 0.06, latent=latent)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
 def test_slots_rising_scores_rescale():
     """Scores that rise by hundreds from tile to tile: the running maximum moves far at every step."""
     base = normal((1, 1, 576), "bf16", 5)
