@@ -742,9 +742,10 @@ void launch_attend(const CUtensorMap& k_map, const CUtensorMap& v_map, const Att
                      v_map, a);
   if (a.ranges == 1) return;
   const unsigned cuts = static_cast<unsigned>(a.ranges - 1), heads = 8 * kTiles;
-  // many parts a segment: one row of 4097 tokens 13 us so, 37 with one warp a head; few:
-  // 64 rows of 1-16 K tokens 15 us more than with one
-  if (a.ranges >= 16 * a.rows * a.segments)
+  // many parts a segment, or few segments: one row of 4097 tokens 13 us so, 37 with one
+  // warp a head, of 512 tokens 9.9 and 11.3, 18 rows of 4097 29.3 and 31.4; else 24 rows
+  // 37.8 and 35.3, 64 rows 74 and 58
+  if (a.ranges >= 16 * a.rows * a.segments || a.rows * a.segments <= 8)
     launch_join(kv8_join_kernel<T, kTiles, 16>, dim3(static_cast<unsigned>(a.rows * a.segments), heads), dim3(512), s, a);
   else
     launch_join(kv8_join_kernel<T, kTiles, 1>, dim3(cuts, heads / 4), dim3(128), s, a);
