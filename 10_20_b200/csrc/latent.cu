@@ -52,6 +52,7 @@
 #include <type_traits>
 
 #include "attention.cuh"
+#include "ranges.cuh"
 #include "sm100.cuh"
 
 namespace v1x {
@@ -89,8 +90,7 @@ struct LatentArgs {
   float* lse;
   float* part;       // [ranges * groups][2][16][latent][4]: four heads' values side by side; then [..][2][2][64] maxima, sums
   float* part_ml;
-  int64_t* where;    // [ranges + 1][4]: where range x begins: the row, its first tile in the line, its
-                     // tiles, and the range's own first tile; [ranges][3]: the number of all tiles
+  RangeBegin* where; // [ranges + 1]
   int32_t* status;
 };
 
@@ -106,7 +106,8 @@ struct LatentShared {
   uint32_t flags[kMaxPairs];
   alignas(16) float factor[kGroup];
   float m[kGroup], l[kGroup];      // of a cluster's CTA
-  int64_t start[4];  // as LatentArgs::where, but [3]: all tiles
+  RangeBegin start;
+  int64_t all;       // tiles
   int64_t cut[2];    // base, extra
   int64_t scan[kThreads / 32 + 1];
   uint32_t tmem;
@@ -145,11 +146,6 @@ __device__ __forceinline__ int64_t slot_of(const LatentArgs& a, int64_t r, int64
     if (a.req) s = s >= 0 && s < a.req_len ? a.req[s] : -1;
   }
   return s >= 0 && s < a.slots ? s : -1;
-}
-
-// The first tile of range x: ranges of `base` units, the first `extra` of them one more.
-__device__ __forceinline__ int64_t range_start(int64_t x, int64_t unit, int64_t base, int64_t extra) {
-  return (x * base + min(x, extra)) * unit;
 }
 
 __device__ __forceinline__ void give_up(LatentShared& sh, int32_t* status) {
@@ -254,10 +250,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     if (tid == 0) {
       const int64_t per = (a.count + kTile - 1) / kTile, t0 = range_start(x, a.unit, a.base, a.extra);
       const int64_t row = kCluster ? x : per ? (t0 >> 31 ? t0 / per : static_cast<uint32_t>(t0) / static_cast<uint32_t>(per)) : 0;
-      sh.start[0] = row;
-      sh.start[1] = row * per;
-      sh.start[2] = per;
-      sh.start[3] = per * a.rows;
+      sh.start = RangeBegin{row, row * per, per, t0};
+      sh.all = per * a.rows;
       sh.cut[0] = a.base;
       sh.cut[1] = a.extra;
     }
@@ -267,41 +261,31 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
     const int64_t beg = min(tid * chunk, a.rows), end = min(beg + chunk, a.rows);
     int64_t mine = 0, all;
     for (int64_t r = beg; r < end; ++r) mine += row_tiles(a, r);
-    int64_t run = block_exclusive_scan(mine, sh.scan, &all);
+    const int64_t run = block_exclusive_scan(mine, sh.scan, &all);
     if (tid == 0) {
-      sh.start[0] = sh.start[1] = 0;
-      sh.start[2] = 1;
-      sh.start[3] = all;
+      sh.all = all;
       sh.cut[0] = all >> 31 ? all / a.ranges : static_cast<uint32_t>(all) / static_cast<uint32_t>(a.ranges);
       sh.cut[1] = all - sh.cut[0] * a.ranges;
     }
     __syncthreads();
     const int64_t t0 = range_start(x, 1, sh.cut[0], sh.cut[1]);
-    if (run <= t0 && t0 < run + mine) {
-      for (int64_t r = beg; r < end; ++r) {
-        const int64_t n = row_tiles(a, r);
-        if (t0 < run + n) {
-          sh.start[0] = r;
-          sh.start[1] = run;
-          sh.start[2] = n;
-          break;
-        }
-        run += n;
-      }
+    if (t0 >= all) {
+      if (tid == 0) sh.start = no_row(t0);
+    } else if (run <= t0 && t0 < run + mine) {
+      sh.start = find_begin(t0, beg, end, run, [&](int64_t r) { return row_tiles(a, r); });
     }
     __syncthreads();
   }
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  const int64_t per = sh.start[2];
+  const int64_t per = sh.start.tiles;
   const int64_t t0 = kCluster ? x * per + per * rank / a.share : range_start(x, a.unit, sh.cut[0], sh.cut[1]);
   const int64_t t1 = kCluster ? x * per + per * (rank + 1) / a.share : range_start(x + 1, a.unit, sh.cut[0], sh.cut[1]);
   const int n = static_cast<int>(t1 - t0);     // tiles of the range
-  Place at{static_cast<int>(sh.start[0]), static_cast<int>(t0 - sh.start[1]), static_cast<int>(sh.start[2])};
+  Place at{static_cast<int>(sh.start.place), static_cast<int>(t0 - sh.start.first), static_cast<int>(sh.start.tiles)};
   if (tid == 0 && group == 0 && a.where) {
-    for (int i = 0; i < 3; ++i) a.where[4 * x + i] = sh.start[i];
-    a.where[4 * x + 3] = t0;
-    if (x == a.ranges - 1) a.where[4 * x + 7] = sh.start[3];
+    a.where[x] = sh.start;
+    if (x == a.ranges - 1) a.where[x + 1].begin = sh.all;
   }
 
   if (warp < 4) {
@@ -738,24 +722,24 @@ __global__ void __launch_bounds__(kShare == 1 ? kLatent / 2 : 32 * kShare) laten
     if (threadIdx.x == 0) found = kMaxCtas;
     __syncthreads();
     for (int i = threadIdx.x + 1; i < a.ranges; i += 32 * kShare)
-      if (a.where[4 * i] == blockIdx.x && a.where[4 * i + 3] > a.where[4 * i + 1]) atomicMin(&found, i);
+      if (a.where[i].place == blockIdx.x && begins_inside(a.where[i])) atomicMin(&found, i);
     __syncthreads();
     x = found;
     if (x == kMaxCtas) return;
   }
-  const int64_t first = a.where[4 * x + 1], begin = a.where[4 * x + 3], before = a.where[4 * x - 1];
-  if (begin == first || before > first) return;              // the whole block
-  const int64_t row = a.where[4 * x], end = first + a.where[4 * x + 2];
+  if (!cuts_first(a.where, x)) return;                       // the whole block
+  const int64_t row = a.where[x].place, first = a.where[x].first, end = first + a.where[x].tiles;
+  const bool earlier = a.where[x - 1].begin < first;
   // the part of range x - 1 + i, which may begin in an earlier row if i is 0
   const int64_t base = (static_cast<int64_t>(x - 1) * a.groups + h / kGroup) * 2, step = 2 * a.groups;
-  auto part = [&](int i) { return base + i * step + (i == 0 && before < first ? 1 : 0); };
-  auto live = [&](int i) { return a.where[4 * (x + i) + 3] > a.where[4 * (x - 1 + i) + 3]; };
+  auto part = [&](int i) { return base + i * step + (i == 0 && earlier ? 1 : 0); };
+  auto live = [&](int i) { return a.where[x + i].begin > a.where[x - 1 + i].begin; };
   auto four = [](const float* p) { return *reinterpret_cast<const float4*>(p); };
   const float* const ml = a.part_ml + h % kGroup;
   float4 m = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
   int parts = 0;
   for (int i = lane; i <= a.ranges - x; i += 32) {
-    if (a.where[4 * (x - 1 + i) + 3] >= end) break;
+    if (a.where[x - 1 + i].begin >= end) break;
     parts = i + 1;
     if (!live(i)) continue;
     const float4 v = four(ml + part(i) * 2 * kGroup);
@@ -924,7 +908,7 @@ extern "C" int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, i
   if (rows <= 0 || heads <= 0 || heads > 1024 || count <= 0 || latent <= 0) return 0;
   const Cut c = cut_for(rows, heads, count, equal != 0);
   if (c.whole || c.ranges == 1) return 0;
-  return (c.ranges + 1) * 32 + c.ranges * ((heads + kGroup - 1) / kGroup) * 2 * kGroup * (latent + 2) * 4;
+  return (c.ranges + 1) * static_cast<int64_t>(sizeof(RangeBegin)) + c.ranges * ((heads + kGroup - 1) / kGroup) * 2 * kGroup * (latent + 2) * 4;
 }
 
 extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, const void* pool, int64_t slots,
@@ -958,8 +942,8 @@ extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, con
                0, static_cast<int>(groups), static_cast<int>(c.ranges), static_cast<int>(c.share), c.unit, c.base, c.extra, scale * kLog2e, out,
                lse, nullptr, nullptr, nullptr, status};
   if (need) {
-    a.where = static_cast<int64_t*>(workspace);
-    a.part = reinterpret_cast<float*>(a.where + 4 * (c.ranges + 1));
+    a.where = static_cast<RangeBegin*>(workspace);
+    a.part = reinterpret_cast<float*>(a.where + c.ranges + 1);
     a.part_ml = a.part + c.ranges * groups * 2 * kGroup * latent;
   }
   V1X_CHECK_ARG(c.unit * (c.base + 1) < (int64_t(1) << 31), "latent_attention: too many tokens for one call");
