@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "attention.cuh"
+#include "ranges.cuh"
 #include "sm100.cuh"
 
 namespace v1x {
@@ -202,8 +203,7 @@ struct AttendArgs {
   float* lse;
   float* part;      // [ranges][2][8 kTiles][128], then [..][2] maxima and sums
   float* part_ml;
-  int64_t* where;   // [ranges + 1][4]: where range x begins: row * segments + segment, that segment's first page in
-                    // the line, its pages, the range's own first page; [ranges][3]: the number of all pages
+  RangeBegin* where;   // [ranges + 1]; tiles are pages, place: row * segments + segment
   int32_t* status;
 };
 
@@ -287,30 +287,22 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const int64_t per = all >> 31 ? all / a.ranges : static_cast<uint32_t>(all) / static_cast<uint32_t>(a.ranges);
   const int64_t extra = all - per * a.ranges;
   const int64_t t0 = x * per + min(x, extra), pages_mine = x < a.ranges ? per + (x < extra ? 1 : 0) : 0;
-  int64_t row = 0, pages = 1, page = 0, segment = 0, first = 0;
-  if (all > 0 && x < a.ranges) {
+  int64_t row = 0, page = 0, segment = 0;
+  RangeBegin range = no_row(t0);               // an empty one stays so
+  if (t0 < all && x < a.ranges) {
     int lo = 0;   // the last thread whose rows begin at or before t0 (those behind it with the same prefix are empty)
     for (int step = kWarps * 16; step > 0; step >>= 1)
       if (lo + step < kWarps * 32 && sh.prefix[lo + step] <= t0) lo += step;
-    int64_t at = sh.prefix[lo];
-    for (row = lo * chunk; row < a.rows; ++row) {
-      const int64_t p = row_pages(a, row), all_of = p * a.segments;
-      if (t0 < at + all_of) {
-        pages = p;
-        segment = (t0 - at) / p;
-        page = t0 - at - segment * p;
-        first = at + segment * p;
-        break;
-      }
-      at += all_of;
-    }
+    range = find_begin(t0, lo * chunk, a.rows, sh.prefix[lo], [&](int64_t r) { return row_pages(a, r) * a.segments; });
+    row = range.place;
+    const int64_t p = row_pages(a, row);
+    segment = (t0 - range.first) / p;
+    page = t0 - range.first - segment * p;
+    range = RangeBegin{row * a.segments + segment, t0 - page, p, t0};
   }
   if (a.where && lane == 0 && x < a.ranges) {
-    a.where[4 * x] = row * a.segments + segment;
-    a.where[4 * x + 1] = first;
-    a.where[4 * x + 2] = pages;
-    a.where[4 * x + 3] = t0;
-    if (x == a.ranges - 1) a.where[4 * x + 7] = all;
+    a.where[x] = range;
+    if (x == a.ranges - 1) a.where[x + 1].begin = all;
   }
 
   // ---- the walk ---------------------------------------------------------------------
@@ -365,7 +357,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     issued &= ~(1u << slot);
   };
 
-  Place now{static_cast<int>(row), static_cast<int>(segment), static_cast<int>(page), static_cast<int>(pages)}, ahead = now;   // ahead: the page whose block was looked up last
+  Place now{static_cast<int>(row), static_cast<int>(segment), static_cast<int>(page), static_cast<int>(range.tiles)}, ahead = now;   // ahead: the page whose block was looked up last
   Block cur{-1, 0, 0}, nxt{-1, 0, 0};
   if (n > 0) {
     cur = block_of(ahead);
@@ -661,24 +653,23 @@ __global__ void __launch_bounds__(kShare == 1 ? 128 : 32 * kShare) kv8_join_kern
     if (threadIdx.x == 0) found = kMaxRanges;
     __syncthreads();
     for (int i = threadIdx.x + 1; i < a.ranges; i += 32 * kShare)
-      if (a.where[4 * i] == blockIdx.x && a.where[4 * i + 3] > a.where[4 * i + 1]) atomicMin(&found, i);
+      if (a.where[i].place == blockIdx.x && begins_inside(a.where[i])) atomicMin(&found, i);
     __syncthreads();
     x = found;
     if (x == kMaxRanges) return;
   }
-  const int64_t first = a.where[4 * x + 1], begin = a.where[4 * x + 3], before = a.where[4 * x - 1];
-  if (begin == first || before > first) return;
-  const int64_t place = a.where[4 * x], end = first + a.where[4 * x + 2];
+  if (!cuts_first(a.where, x)) return;
+  const int64_t place = a.where[x].place, first = a.where[x].first, end = first + a.where[x].tiles;
   const int64_t row = place / a.segments, segment = place - row * a.segments;
   const int group = static_cast<int>(segment % a.groups), hg = kShare == 1 ? blockIdx.y * 4 + warp : blockIdx.y;
   if (hg >= min(kHeads, a.per_kv - group * kHeads)) return;   // kShare > 1: the whole block
   const int64_t h = segment / a.groups * a.per_kv + group * kHeads + hg;
-  const int64_t shift = before < first ? kHeads : 0;
+  const int64_t shift = a.where[x - 1].begin < first ? kHeads : 0;
   auto part = [&](int i) { return static_cast<int64_t>(x - 1 + i) * 2 * kHeads + hg + (i == 0 ? shift : 0); };
   float m = -CUDART_INF_F, l = 0.0f;
   int parts = 0;
   for (int i = lane; i <= a.ranges - x; i += 32) {
-    const int64_t t0 = a.where[4 * (x - 1 + i) + 3], t1 = a.where[4 * (x + i) + 3];
+    const int64_t t0 = a.where[x - 1 + i].begin, t1 = a.where[x + i].begin;
     if (t0 >= end) break;
     parts = i + 1;
     if (t1 > t0) m = fmaxf(m, a.part_ml[2 * part(i)]);
@@ -692,7 +683,7 @@ __global__ void __launch_bounds__(kShare == 1 ? 128 : 32 * kShare) kv8_join_kern
   float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 8
   for (int i = kShare == 1 ? 0 : warp; i < parts; i += kShare) {
-    if (a.where[4 * (x + i) + 3] == a.where[4 * (x - 1 + i) + 3]) continue;
+    if (a.where[x + i].begin == a.where[x - 1 + i].begin) continue;
     const float w = exp2f(a.part_ml[2 * part(i)] - ref);
     l += a.part_ml[2 * part(i) + 1] * w;
     const float4 v = *reinterpret_cast<const float4*>(a.part + part(i) * 128 + 4 * lane);
@@ -804,7 +795,7 @@ extern "C" int64_t v1x_kv8_attend_workspace(int64_t rows, int64_t heads, int64_t
   using namespace v1x;
   if (rows <= 0 || kv_heads <= 0 || heads <= 0 || heads > 1024 || heads % kv_heads || table_pages <= 0) return 0;
   const Plan p = plan_for(rows, heads, kv_heads, table_pages);
-  return p.ranges == 1 ? 0 : (p.ranges + 1) * 32 + p.ranges * 2 * 8 * p.tiles * (128 + 2) * 4;
+  return p.ranges == 1 ? 0 : (p.ranges + 1) * static_cast<int64_t>(sizeof(RangeBegin)) + p.ranges * 2 * 8 * p.tiles * (128 + 2) * 4;
 }
 
 extern "C" int v1x_kv8_attend(const void* q, int64_t qs0, int64_t qs1, const uint8_t* k_cache, const float* k_scale,
@@ -839,8 +830,8 @@ extern "C" int v1x_kv8_attend(const void* q, int64_t qs0, int64_t qs1, const uin
                static_cast<int>(heads / kv_heads), static_cast<int>(p.groups), static_cast<int>(p.segments),
                static_cast<int>(p.ranges), scale * kLog2e, out, lse, nullptr, nullptr, nullptr, status};
   if (p.ranges > 1) {
-    a.where = static_cast<int64_t*>(workspace);
-    a.part = reinterpret_cast<float*>(a.where + 4 * (p.ranges + 1));
+    a.where = static_cast<RangeBegin*>(workspace);
+    a.part = reinterpret_cast<float*>(a.where + p.ranges + 1);
     a.part_ml = a.part + p.ranges * 2 * 8 * p.tiles * 128;
   }
   CUtensorMap k_map = {}, v_map = {};

@@ -15,6 +15,7 @@ from test_gpu_attention import DEV, check, ints, normal, want_slots
 pytestmark = pytest.mark.gpu
 
 L = importlib.import_module("10_20_b200.latent_attention")
+K = importlib.import_module("10_20_b200.kv8")
 
 
 def poison(size):
@@ -71,3 +72,34 @@ def test_pages_totals_around_the_ranges(total):
     pages_case([64 * total, 0, 0], 150, 3, latent=128)
     lens = [64 if i < total else 0 for i in range(160)]
     pages_case(lens[::-1], 2, 3, latent=128)
+
+
+def attend_case(lens, width, kv_heads, heads, dtype="bf16"):
+    rows = len(lens)
+    c = T.new_cache(rows * width + 1, kv_heads)
+    table = np.random.default_rng(11).permutation(rows * width + 1)[:rows * width].reshape(rows, width).astype(np.int32)
+    T.fill(c, table, lens, 12)
+    q = normal((rows, heads, 128), dtype, 13)
+    out, lse, o, l = guarded(rows, heads, 128, q.dtype, max(2, 600 - rows))
+    poison(K.workspace_bytes(rows, heads, kv_heads, width))
+    K.attend(q, *c, ints(table), ints(lens), 0.09, out=o, lse=l)
+    check(o, l, T.want_attend(q, c, table, lens, 0.09, dtype), (lens, width, kv_heads, heads))
+    assert untouched(out, lse, rows)
+
+
+@pytest.mark.parametrize("heads", [1, 8, 16])
+@pytest.mark.parametrize("n", [1, 63, 64])
+@pytest.mark.parametrize("rows,at,width", [(1, 0, 2), (9, 4, 2), (16, 0, 8), (16, 9, 8), (16, 15, 8), (301, 200, 4)])
+def test_attend_one_page_of_a_padded_batch(rows, at, width, n, heads):
+    """One K/V head and one row that is not empty: a single page of work, both joins."""
+    lens = [0] * rows
+    lens[at] = n
+    attend_case(lens, width, 1, heads)
+
+
+@pytest.mark.parametrize("kv_heads,heads", [(1, 5), (2, 8), (1, 40), (8, 8)])
+@pytest.mark.parametrize("total", [0, 1, 2, 3])
+def test_attend_few_pages(total, kv_heads, heads):
+    attend_case([64 * total] + [0] * 11, 5, kv_heads, heads, "fp16")
+    attend_case([0] * (12 - total) + [64] * total, 2, kv_heads, heads)
+    attend_case([0, 64 * total - 1 if total else 0, 0], 30, kv_heads, heads)
