@@ -5,6 +5,7 @@
 
 #include "attention.cuh"
 #include "ranges.cuh"
+#include "ring.cuh"
 #include "sm100.cuh"
 
 namespace v1x {
@@ -337,24 +338,22 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   };
   const uint32_t ring = smem_u32(base + warp * kRing * kPageBytes8);
   uint64_t* const full = sh.full[warp];
-  uint32_t phases = 0, issued = 0;             // per buffer: the phase that the next wait is for; a load is in flight
+  RingState state;
   auto load = [&](const CUtensorMap* map, int slot, int at) {
-    if (at < 0) return;
-    issued |= 1u << slot;
+    if (at < 0 || !state.start(slot)) return;
     if (lane == 0) {
       mbar_arrive_expect_tx(&full[slot], kPageBytes8);
       tma_load_2d(base + (warp * kRing + slot) * kPageBytes8, map, &full[slot], 0, at * 64);
     }
   };
-  bool ok = true;
   auto arrived = [&](int slot) {
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], (phases >> slot) & 1, &sh.abort, kWaitNs))) {
-      ok = false;
+    const bool done = __all_sync(0xffffffffu, mbar_wait(&full[slot], state.phase(slot), &sh.abort, kWaitNs));
+    if (!done) {
       *reinterpret_cast<volatile int*>(&sh.abort) = 1;
       if (a.status) atomicExch(a.status, V1X_STATUS_TIMEOUT);
     }
-    phases ^= 1u << slot;
-    issued &= ~(1u << slot);
+    state.waited(slot, done);
+    return done;
   };
 
   Place now{static_cast<int>(row), static_cast<int>(segment), static_cast<int>(page), static_cast<int>(range.tiles)}, ahead = now;   // ahead: the page whose block was looked up last
@@ -375,7 +374,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   bool fresh = true;
   int parts = 0;
   int slot = 0;                                // of the page's keys; its values follow
-  for (int it = 0; it < n && ok; ++it) {
+  for (int it = 0; it < n; ++it) {
     const int kv = now.segment / a.groups, group = now.segment % a.groups;
     const int heads = min(kHeads, a.per_kv - group * kHeads);
     const int head0 = kv * a.per_kv + group * kHeads;
@@ -443,7 +442,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[t][j][i] = 0.0f;
-      arrived(slot);
+      if (!arrived(slot)) break;
       const uint32_t k = ring + slot * kPageBytes8;
       // token tiles j innermost: their sums are independent, one's next step waits 20 cycles
       const uint32_t r0 = k + g * 128;         // tokens 16 j + g, + 8: the same row & 7
@@ -516,7 +515,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
                          : "=r"(p[t][2 * j + y])
                          : "r"(pack2<__half>(s[t][j][2 * y], s[t][j][2 * y + 1])));
       }
-      arrived(vslot);
+      if (!arrived(vslot)) break;
       const uint32_t v = ring + vslot * kPageBytes8;
       // a lane's 16 columns in kPasses parts: two tiles' sums of all 16 would not fit the
       // registers beside the rest
@@ -622,9 +621,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     nxt = far;
     slot = vslot + 1 == kRing ? 0 : vslot + 1;
   }
-  if (!ok)   // what is in flight lands before the CTA ends
+  if (!state.ok)   // what is under way lands before the CTA ends
     for (int i = 0; i < kRing; ++i)
-      if (issued >> i & 1) mbar_wait(&full[i], (phases >> i) & 1, &sh.zero, kWaitNs);
+      if (state.under_way(i)) mbar_wait(&full[i], state.phase(i), &sh.zero, kWaitNs);
   // ---- rows that have no page ----------------------------------------------------------
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     if (row_pages(a, r) > 0) continue;

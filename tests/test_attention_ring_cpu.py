@@ -1,0 +1,110 @@
+"""CPU: the 8-bit attention's ring of buffers when a wait gives up (csrc/ring.cuh).
+
+A program built from the header walks pages as a warp does -- keys, values and the next
+page's keys in three buffers, some pages outside the cache -- over barriers that count
+boxes, with every wait in turn giving up while its box is still under way.  No box may
+be sent to a buffer that waits for one, every wait has to be for the phase of the box
+under way, and all boxes have to have landed at the end."""
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "10_20_b200" / "csrc"
+
+PROGRAM = r"""
+#include <cstdio>
+#include <vector>
+
+#include "ring.cuh"
+
+using v1x::attn::RingState;
+
+static int bad = 0;
+
+struct Barriers {
+  int landed[3] = {0, 0, 0};
+  bool flying[3] = {false, false, false};
+  int waits = 0, give_up_at;
+  explicit Barriers(int at) : give_up_at(at) {}
+  void send(int slot) {
+    if (flying[slot]) ++bad;      // two boxes in one phase
+    flying[slot] = true;
+  }
+  bool wait(int slot, unsigned parity, bool drain) {
+    if (!flying[slot] || parity != (landed[slot] & 1u)) {
+      ++bad;                      // a wait that no box ends, or for another phase
+      return true;
+    }
+    if (!drain && waits++ >= give_up_at) return false;   // this warp's, and every later one's
+    flying[slot] = false;
+    ++landed[slot];
+    return true;
+  }
+};
+
+// here[i]: page i is in the cache
+static int walk(const std::vector<bool>& here, int give_up_at, bool leave) {
+  Barriers b(give_up_at);
+  RingState ring;
+  const int n = here.size();
+  auto load = [&](int slot, int page) {
+    if (page >= n || !here[page] || !ring.start(slot)) return;
+    b.send(slot);
+  };
+  auto arrived = [&](int slot) {
+    const bool done = b.wait(slot, ring.phase(slot), false);
+    ring.waited(slot, done);
+    return done;
+  };
+  load(0, 0);
+  load(1, 0);
+  load(2, 1);
+  for (int it = 0, slot = 0; it < n && ring.ok; ++it) {
+    const int vslot = (slot + 1) % 3;
+    if (here[it]) {
+      if (!arrived(slot) && leave) break;
+      load(slot, it + 1);
+      if (ring.ok && !arrived(vslot) && leave) break;
+    } else {
+      load(slot, it + 1);
+    }
+    load(vslot, it + 2);
+    slot = (vslot + 1) % 3;
+  }
+  if (!ring.ok)
+    for (int i = 0; i < 3; ++i)
+      if (ring.under_way(i)) b.wait(i, ring.phase(i), true);
+  for (int i = 0; i < 3; ++i)
+    if (b.flying[i]) ++bad;       // lands after its CTA
+  return b.waits;
+}
+
+int main() {
+  for (int n = 1; n <= 9; ++n)
+    for (int mask = 0; mask < 1 << n; ++mask) {
+      std::vector<bool> here(n);
+      for (int i = 0; i < n; ++i) here[i] = mask >> i & 1;
+      const int waits = walk(here, 1 << 20, true);
+      for (int at = 0; at < waits; ++at)
+        for (bool leave : {true, false}) walk(here, at, leave);
+    }
+  std::printf("%d faults\n", bad);
+  return bad != 0;
+}
+"""
+
+
+def test_a_wait_that_gives_up_leaves_no_box_behind(tmp_path):
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        pytest.skip("no host compiler")
+    source = tmp_path / "ring.cpp"
+    source.write_text(PROGRAM)
+    program = tmp_path / "ring"
+    built = subprocess.run([cxx, "-std=c++17", "-O1", "-x", "c++", "-I", str(CSRC), str(source), "-o", str(program)],
+                           capture_output=True, text=True)
+    assert built.returncode == 0, built.stderr
+    ran = subprocess.run([str(program)], capture_output=True, text=True, timeout=120)
+    assert ran.returncode == 0, ran.stdout
