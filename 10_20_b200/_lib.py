@@ -33,6 +33,7 @@ F32 = ctypes.c_float
 SIGNATURES = {
     "v1x_version": [],
     "v1x_last_error": [],
+    "v1x_status_word": [P],
     "v1x_route": [P, I64, I64, P, P, P, I32, I64, I64, P, P, I64, P, I64, I32, I64, P],
     "v1x_topk": [P, I64, I64, P, P, I64, P, P, I64, P, I32, I64, P, P, P, P, P, I64, I64, I32, P,
                  I64, I32, I32, P, I64, I32, I64, P],

@@ -51,7 +51,24 @@ int num_sms() {
   return sms;
 }
 
+// The library's status word, one per device since a module's variables are: 0 at first.
+__device__ int32_t g_status_word;
+
 }  // namespace v1x
+
+extern "C" int v1x_status_word(int32_t** word) {
+  using namespace v1x;
+  clear_error();
+  V1X_CHECK_ARG(word != nullptr, "status_word: NULL argument");
+  void* p = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&p, g_status_word);
+  if (e != cudaSuccess) {
+    set_error("v1x_status_word: %s", cudaGetErrorString(e));
+    return V1X_ERR_CUDA;
+  }
+  *word = static_cast<int32_t*>(p);
+  return V1X_OK;
+}
 
 extern "C" int v1x_version(void) { return 0x000100; }
 

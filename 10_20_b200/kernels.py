@@ -21,6 +21,7 @@ inside capture, call :func:`check_status` after the graph runs.
 """
 from __future__ import annotations
 
+import ctypes
 import threading
 
 import torch
@@ -35,31 +36,40 @@ class ArenaExhausted(RuntimeError):
 
 _status_lock = threading.Lock()
 _status: dict[int, torch.Tensor] = {}
+_status_address: dict[int, int] = {}
+
+
+class _Word:
+    """One int32 at a device address, as torch.as_tensor takes it."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 3}
 
 
 def status_word(device: torch.device) -> torch.Tensor:
-    """The per-device int32 status word the page-lifecycle kernels report into."""
+    """The per-device int32 status word the kernels report into."""
     idx = torch.device(device).index or 0
     with _status_lock:
         t = _status.get(idx)
         if t is None:
+            dev = torch.device("cuda", idx)
             # a normal tensor even when first asked for under inference mode, so
             # that check_status can reset it anywhere
             with torch.inference_mode(False):
-                t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+                t = torch.as_tensor(_Word(status_ptr(dev)), device=dev)
             _status[idx] = t
     return t
 
 
-def status_ptr(device: torch.device) -> int | None:
-    """The status word's address for a call whose waits report into it; None where it is first
-    asked for inside a graph capture, which would record its allocation and zeroing instead."""
-    t = _status.get(device.index)
-    if t is None:
-        if torch.cuda.is_current_stream_capturing():
-            return None
-        t = status_word(device)
-    return t.data_ptr()
+def status_ptr(device: torch.device) -> int:
+    """The status word's address.  The word is a variable of the library, neither allocated nor
+    zeroed by a launch, so that a call inside a graph capture may be the first to ask for it."""
+    address = _status_address.get(device.index)
+    if address is None:
+        p = ctypes.c_void_p()
+        _lib.call("v1x_status_word", ctypes.byref(p), device=device)
+        address = _status_address[device.index] = p.value
+    return address
 
 
 def check_status(device=None, reset: bool = True):

@@ -59,6 +59,11 @@ V1X_API int v1x_version(void);
 /* Message of the last failed call on this thread ("" if none). */
 V1X_API const char* v1x_last_error(void);
 
+/* *word: the address, on the current device, of a status word that lives as long as
+ * the library: i32, 0 at first, for the `status` arguments below.  Nothing is allocated
+ * and nothing launched, so it may also be asked for inside a stream capture. */
+V1X_API int v1x_status_word(int32_t** word);
+
 /* ------------------------------------------------------------------------ */
 /* fused.route -- replaces V1QueryKernel::route (VQ:155-180, kernel VQ:7-49).
  * scores  f32 [batch, score_cols] with row stride score_stride (% 4 == 0)
