@@ -269,12 +269,18 @@ class SelectionStep:
 
     def algorithmic_bytes(self) -> dict:
         """Compulsory bytes of one step, each input byte once, each output once
-        (the per-request sum of `sharding.row_bytes`)."""
+        (the per-request sum of `sharding.row_bytes`); "attend" only with
+        attention."""
         c = self.case
         row = c.latent.shape[-1] * c.latent.element_size() if self.gather else 0
+        attend = None
+        if self.attention is not None:
+            q, (out, lse) = self.attention[0], self.attended
+            attend = (c.latent.shape[-1] * c.latent.element_size(),
+                      sum(t[0].numel() * t.element_size() for t in (q, out, lse)))
         total = {}
         for n in c.lens.tolist():
             for k, v in row_bytes(n, c.H, c.take, c.window, c.topk, row, 2 if self.gather_v else 1,
-                                  staging=not self.fused_select).items():
+                                  staging=not self.fused_select, attend=attend).items():
                 total[k] = total.get(k, 0) + v
         return total

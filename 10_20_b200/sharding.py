@@ -13,14 +13,17 @@ import heapq
 
 
 def row_bytes(n: int, heads: int, take: int, window: int, topk: int, latent_row_bytes: int = 0,
-              outputs: int = 1, staging: bool = True) -> dict:
+              outputs: int = 1, staging: bool = True, attend=None) -> dict:
     """Compulsory bytes of one request of token length n (each input byte once,
     each output byte once): q/w, centre keys (132 B per centre, 8 per built
     page), sink/tail staging (read + write; only for the operator sequence that
     copies those keys into the fine pool -- the fused selection scores them in
     place, `staging=False`), fine keys (selected pages and the sink/tail
     tokens) + members of the selected pages, the three int32 Top-k outputs and
-    the latent gather (read once, written `outputs` times)."""
+    the latent gather (read once, written `outputs` times).  attend: (bytes of a
+    latent row, bytes of the request's queries and attended outputs) where the step
+    attends the selected rows instead, of which there are at most topk, n and the
+    candidates."""
     pages = max(n - 1, 0) // 1024 * 16
     tk = min(pages, take)
     sink = min(64, n)
@@ -32,8 +35,10 @@ def row_bytes(n: int, heads: int, take: int, window: int, topk: int, latent_row_
     fine = (tk * 64 + count) * 132 + tk * 64 * 4
     out = topk * 4 * 3
     gather = topk * latent_row_bytes * (1 + outputs) if latent_row_bytes else 0
-    return dict(q=q, centres=centres, staging=staging, fine=fine, topk_out=out, gather=gather,
-                total=q + centres + staging + fine + out + gather)
+    parts = dict(q=q, centres=centres, staging=staging, fine=fine, topk_out=out, gather=gather)
+    if attend is not None:
+        parts["attend"] = min(topk, n, tk * 64 + count) * attend[0] + attend[1]
+    return dict(parts, total=sum(parts.values()))
 
 
 def shard_requests(costs, world: int, per_rank: int | None = None):
