@@ -93,7 +93,8 @@ def workspace_bytes(rows, heads, count, latent, equal) -> int:
     return _lib.lib().v1x_latent_attention_workspace(rows, heads, count, latent, equal)
 
 
-def _absorbed(q, pool, request_slots, index, count, lens, scale, latent, out, lse):
+def check_absorbed(q, pool, scale, latent: int = 512) -> tuple[int, float]:
+    """What every absorbed call requires of its queries, pool and scale; the type's code and the scale."""
     code = _DTYPES.get(q.dtype)
     require(code is not None and q.dim() == 3, "q: [rows, heads, dim] bfloat16 or float16")
     rows, heads, dim = q.shape
@@ -105,6 +106,12 @@ def _absorbed(q, pool, request_slots, index, count, lens, scale, latent, out, ls
     require(_rows16(q) and _rows16(pool), "q, pool: unit inner stride, rows 16-byte aligned")
     scale = float(scale)
     require(math.isfinite(scale), "scale: a finite number")
+    return code, scale
+
+
+def _absorbed(q, pool, request_slots, index, count, lens, scale, latent, out, lse):
+    code, scale = check_absorbed(q, pool, scale, latent)
+    rows, heads, dim = q.shape
     require(q.is_cuda, "q must be a CUDA tensor (there is no CPU path)")
     device = q.device
     _one_device(device, pool, request_slots, index, lens, out, lse)

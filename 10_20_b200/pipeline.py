@@ -35,7 +35,7 @@ from . import _lib
 from . import kernels as K
 from . import query_fused, scoring
 from .gather import _gather_impl
-from .latent_attention import attend_slots, workspace_bytes
+from .latent_attention import attend_slots, check_absorbed, workspace_bytes
 from .sharding import row_bytes
 
 
@@ -60,8 +60,11 @@ class SelectionStep:
         grid (for small batches stepped many at a time).  attention: (q, scale)
         -- each run then attends the absorbed queries q [B, heads, D] over the
         selected rows of the latent pool where they lie
-        (latent_attention.attend_slots, the first 512 of D the values), after the
-        selection; `attended` holds (out, lse).  q is read at every run."""
+        (latent_attention.attend_slots, the first 512 of D the values, so D is 512
+        or 576), after the selection; `attended` holds (out, lse).  q is read at
+        every run.  A bounded wait that gives up is reported in `status` by the
+        one-launch selection, and in the device's status word
+        (kernels.check_status) by the scorers and the attention."""
         c = self.case = case
         d = c.lens.device
         B = c.B
@@ -117,7 +120,9 @@ class SelectionStep:
         self.attention = attention
         if attention is not None:
             _lib.require(c.latent is not None, "attention needs a case with a latent pool")
-            aq = attention[0]
+            aq, scale = attention
+            check_absorbed(aq, c.latent, scale)
+            _lib.require(aq.shape[0] == B and aq.device == d, "attention: a query row per request, on the case's device")
             self.attended = (torch.empty((B, aq.shape[1], 512), dtype=aq.dtype, device=d),
                              torch.empty((B, aq.shape[1]), dtype=torch.float32, device=d))
 
