@@ -111,6 +111,9 @@ inline void launch_join(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStr
 }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// A scale that is finite, also times log2 e (NaN is not).
+inline bool scale_in_range(float scale) { return scale > -0x1p127f && scale < 0x1p127f; }
+
 __host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace attn

@@ -813,6 +813,7 @@ extern "C" int v1x_kv8_attend(const void* q, int64_t qs0, int64_t qs1, const uin
                   reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
                     (qs0 | qs1) % 8 == 0,
                 "kv8_attend: the caches and the rows of q and out must be 16-byte aligned");
+  V1X_CHECK_ARG(scale_in_range(scale), "kv8_attend: the scale must be finite and below 2^127");
   if (rows == 0) return V1X_OK;
   V1X_CHECK_ARG(q && out && lse && lens && (table || table_pages == 0) &&
                     ((k_cache && k_scale && v_cache && v_scale) || pages == 0),

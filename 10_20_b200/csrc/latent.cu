@@ -929,6 +929,7 @@ extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, con
   V1X_CHECK_ARG(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pool) |
                   reinterpret_cast<uintptr_t>(out)) & 15) == 0 && qs0 % 8 == 0 && qs1 % 8 == 0 && pool_stride % 8 == 0,
                 "latent_attention: q, pool and out rows must be 16-byte aligned");
+  V1X_CHECK_ARG(scale_in_range(scale), "latent_attention: the scale must be finite and below 2^127");
   V1X_CHECK_ARG(!lens || (count % 64 == 0 && !req), "latent_attention: a page table takes whole pages and no slot map");
   if (rows == 0) return V1X_OK;
   V1X_CHECK_ARG(q && out && lse && (index || count == 0) && (pool || slots == 0), "latent_attention: NULL argument");

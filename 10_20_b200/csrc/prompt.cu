@@ -516,6 +516,7 @@ extern "C" int v1x_prompt_attention(const void* q, int64_t qs0, int64_t qs1, con
                   reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
                     (qs0 | qs1 | ks0 | ks1 | krs0 | vs0 | vs1) % 8 == 0,
                 "prompt_attention: q, k, k_rope, v and out rows must be 16-byte aligned");
+  V1X_CHECK_ARG(scale_in_range(scale), "prompt_attention: the scale must be finite and below 2^127");
   if (tokens == 0 || requests == 0) return V1X_OK;
   V1X_CHECK_ARG(q && out && lse && offsets && kv_offsets && ((k && v) || keys == 0), "prompt_attention: NULL argument");
   // a masked score, -inf, has to stay -inf under the scale, so that is never 0

@@ -21,14 +21,13 @@ as ``latent_attention`` does.
 from __future__ import annotations
 
 import functools
-import math
 
 import torch
 
 from . import _lib
 from ._lib import ptr, require
 from .kernels import status_ptr
-from .latent_attention import PAGE, _DTYPES, _index, _one_device, _outputs, _rows16, _step
+from .latent_attention import MAX_SCALE, PAGE, _DTYPES, _index, _one_device, _outputs, _rows16, _step
 
 
 def _cache(k_cache, k_scale, v_cache, v_scale):
@@ -97,7 +96,7 @@ def attend(q, k_cache, k_scale, v_cache, v_scale, table, lens, scale, out=None, 
     require(lens.dtype is torch.int32 and lens.shape == (rows,) and lens.is_contiguous(),
             "lens: contiguous int32 [rows]")
     scale = float(scale)
-    require(math.isfinite(scale), "scale: a finite number")
+    require(abs(scale) < MAX_SCALE, "scale: a finite number below 2^127")
     require(q.is_cuda, "q must be a CUDA tensor (there is no CPU path)")
     device = q.device
     _one_device(device, k_cache, k_scale, v_cache, v_scale, table, lens, out, lse)

@@ -32,7 +32,6 @@ kernel that runs out (2 s) is reported in the device's status word, which
 from __future__ import annotations
 
 import functools
-import math
 
 import torch
 
@@ -41,6 +40,7 @@ from ._lib import ptr, require
 from .kernels import status_ptr
 
 PAGE = 64                                           # tokens per page of the native pool
+MAX_SCALE = 2.0 ** 127                              # so that scale * log2 e is finite in 32 bits
 _DTYPES = {torch.bfloat16: 1, torch.float16: 2}     # codes shared with v1x_pack_q
 
 
@@ -105,7 +105,7 @@ def check_absorbed(q, pool, scale, latent: int = 512) -> tuple[int, float]:
     require(1 <= heads <= 1024, "heads: 1 to 1024")
     require(_rows16(q) and _rows16(pool), "q, pool: unit inner stride, rows 16-byte aligned")
     scale = float(scale)
-    require(math.isfinite(scale), "scale: a finite number")
+    require(abs(scale) < MAX_SCALE, "scale: a finite number below 2^127")
     return code, scale
 
 
@@ -181,7 +181,7 @@ def attend_prompt(q, k, k_rope, v, offsets, scale, kv_offsets=None, out=None, ls
             "q, k, k_rope, v: one type, unit inner stride, rows 16-byte aligned")
     require(1 <= heads <= 1024, "heads: 1 to 1024")
     scale = float(scale)
-    require(math.isfinite(scale), "scale: a finite number")
+    require(abs(scale) < MAX_SCALE, "scale: a finite number below 2^127")
     if kv_offsets is None:
         kv_offsets = offsets
     require(offsets.dtype is torch.int32 and kv_offsets.dtype is torch.int32 and offsets.dim() == 1

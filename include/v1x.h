@@ -651,7 +651,7 @@ V1X_API int v1x_gather_slots(const void* k, const void* v, const int32_t* req, c
  * q [rows, heads, dim] with strides qs0, qs1; pool [slots, dim] with row stride
  * pool_stride; out [rows, heads, latent] contiguous; dtype of q, pool and out: 1
  * bf16, 2 f16; every address and stride a multiple of 16 bytes.  latent in {128,
- * 256, 384, 512}, dim - latent in {0, 64}, heads <= 1024.  workspace: device
+ * 256, 384, 512}, dim - latent in {0, 64}, heads <= 1024, |scale| < 2^127.  workspace: device
  * memory of at least v1x_latent_attention_workspace(rows, heads, count, latent,
  * lens == NULL) bytes, 16-byte aligned, of no meaning before or after the call
  * (NULL if 0 bytes).  status: optional device word for V1X_STATUS_TIMEOUT. */
@@ -669,8 +669,8 @@ V1X_API int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, const 
  * i-th query of nq sees the first i + 1 + nk - nq keys of its nk:
  *   s[i, j] = scale * (q[i, h, 0:128] . k[j, h, :] + q[i, h, 128:128+dr] . k_rope[j, :])
  * out [tokens, heads, 128] and lse [tokens, heads], contiguous; rows of no request
- * are not written.  dr 0 (k_rope NULL) or 64; k, v rows of 128.  Types, alignment
- * and status as above. */
+ * are not written.  dr 0 (k_rope NULL) or 64; k, v rows of 128; tokens / 256 +
+ * requests <= 65535.  Types, alignment, scale and status as above. */
 V1X_API int v1x_prompt_attention(const void* q, int64_t qs0, int64_t qs1, const void* k, int64_t ks0, int64_t ks1,
                   const void* k_rope, int64_t krs0, const void* v, int64_t vs0, int64_t vs1,
                   const int32_t* offsets, const int32_t* kv_offsets, int64_t requests, int64_t tokens,
@@ -696,7 +696,7 @@ V1X_API int v1x_kv8_store(uint8_t* k_cache, float* k_scale, uint8_t* v_cache, fl
  * table_pages) tokens of row r in that cache, heads / kv_heads query heads per K/V
  * head; out [rows, heads, 128] in q's type and lse [rows, heads] contiguous.  A page
  * outside the cache holds no tokens.  pages * kv_heads < 2^25, table_pages < 2^25, rows *
- * kv_heads * table_pages <= 2^34.  workspace and status as in v1x_latent_attention. */
+ * kv_heads * table_pages <= 2^34.  workspace, scale and status as in v1x_latent_attention. */
 V1X_API int64_t v1x_kv8_attend_workspace(int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_pages);
 V1X_API int v1x_kv8_attend(const void* q, int64_t qs0, int64_t qs1, const uint8_t* k_cache, const float* k_scale,
                   const uint8_t* v_cache, const float* v_scale, int64_t pages, int64_t kv_heads,
