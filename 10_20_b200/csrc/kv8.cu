@@ -338,6 +338,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   };
   const uint32_t ring = smem_u32(base + warp * kRing * kPageBytes8);
   uint64_t* const full = sh.full[warp];
+  // After a wait that gave up the warp ends its page, whose result is of no use, and its
+  // walk; `state` keeps it from sending boxes.  (Leaving the page at once made 16 heads a
+  // K/V head 168 us instead of 158: other spills.)
   RingState state;
   auto load = [&](const CUtensorMap* map, int slot, int at) {
     if (at < 0 || !state.start(slot)) return;
@@ -353,7 +356,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       if (a.status) atomicExch(a.status, V1X_STATUS_TIMEOUT);
     }
     state.waited(slot, done);
-    return done;
   };
 
   Place now{static_cast<int>(row), static_cast<int>(segment), static_cast<int>(page), static_cast<int>(range.tiles)}, ahead = now;   // ahead: the page whose block was looked up last
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   bool fresh = true;
   int parts = 0;
   int slot = 0;                                // of the page's keys; its values follow
-  for (int it = 0; it < n; ++it) {
+  for (int it = 0; it < n && state.ok; ++it) {
     const int kv = now.segment / a.groups, group = now.segment % a.groups;
     const int heads = min(kHeads, a.per_kv - group * kHeads);
     const int head0 = kv * a.per_kv + group * kHeads;
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[t][j][i] = 0.0f;
-      if (!arrived(slot)) break;
+      arrived(slot);
       const uint32_t k = ring + slot * kPageBytes8;
       // token tiles j innermost: their sums are independent, one's next step waits 20 cycles
       const uint32_t r0 = k + g * 128;         // tokens 16 j + g, + 8: the same row & 7
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
                          : "=r"(p[t][2 * j + y])
                          : "r"(pack2<__half>(s[t][j][2 * y], s[t][j][2 * y + 1])));
       }
-      if (!arrived(vslot)) break;
+      arrived(vslot);
       const uint32_t v = ring + vslot * kPageBytes8;
       // a lane's 16 columns in kPasses parts: two tiles' sums of all 16 would not fit the
       // registers beside the rest

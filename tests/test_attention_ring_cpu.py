@@ -2,7 +2,8 @@
 
 A program built from the header walks pages as a warp does -- keys, values and the next
 page's keys in three buffers, some pages outside the cache -- over barriers that count
-boxes, with every wait in turn giving up while its box is still under way.  No box may
+boxes, with every wait in turn giving up while its box is still under way, and later
+ones giving up too or not.  The warp ends its page, or leaves it at once.  No box may
 be sent to a buffer that waits for one, every wait has to be for the phase of the box
 under way, and all boxes have to have landed at the end."""
 import shutil
@@ -27,7 +28,8 @@ struct Barriers {
   int landed[3] = {0, 0, 0};
   bool flying[3] = {false, false, false};
   int waits = 0, give_up_at;
-  explicit Barriers(int at) : give_up_at(at) {}
+  bool later;
+  Barriers(int at, bool later) : give_up_at(at), later(later) {}
   void send(int slot) {
     if (flying[slot]) ++bad;      // two boxes in one phase
     flying[slot] = true;
@@ -37,7 +39,10 @@ struct Barriers {
       ++bad;                      // a wait that no box ends, or for another phase
       return true;
     }
-    if (!drain && waits++ >= give_up_at) return false;   // this warp's, and every later one's
+    if (!drain) {
+      const int n = waits++;
+      if (n == give_up_at || (later && n > give_up_at)) return false;
+    }
     flying[slot] = false;
     ++landed[slot];
     return true;
@@ -45,8 +50,8 @@ struct Barriers {
 };
 
 // here[i]: page i is in the cache
-static int walk(const std::vector<bool>& here, int give_up_at, bool leave) {
-  Barriers b(give_up_at);
+static int walk(const std::vector<bool>& here, int give_up_at, bool leave, bool later) {
+  Barriers b(give_up_at, later);
   RingState ring;
   const int n = here.size();
   auto load = [&](int slot, int page) {
@@ -66,7 +71,7 @@ static int walk(const std::vector<bool>& here, int give_up_at, bool leave) {
     if (here[it]) {
       if (!arrived(slot) && leave) break;
       load(slot, it + 1);
-      if (ring.ok && !arrived(vslot) && leave) break;
+      if (!arrived(vslot) && leave) break;
     } else {
       load(slot, it + 1);
     }
@@ -86,9 +91,10 @@ int main() {
     for (int mask = 0; mask < 1 << n; ++mask) {
       std::vector<bool> here(n);
       for (int i = 0; i < n; ++i) here[i] = mask >> i & 1;
-      const int waits = walk(here, 1 << 20, true);
+      const int waits = walk(here, 1 << 20, true, true);
       for (int at = 0; at < waits; ++at)
-        for (bool leave : {true, false}) walk(here, at, leave);
+        for (bool leave : {true, false})
+          for (bool later : {true, false}) walk(here, at, leave, later);
     }
   std::printf("%d faults\n", bad);
   return bad != 0;
