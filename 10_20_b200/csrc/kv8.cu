@@ -204,7 +204,7 @@ struct AttendArgs {
   float* lse;
   float* part;      // [ranges][2][8 kTiles][128], then [..][2] maxima and sums
   float* part_ml;
-  RangeBegin* where;   // [ranges + 1]; tiles are pages, place: row * segments + segment
+  int64_t* where;   // [ranges + 1][4]: the ranges' records; tiles are pages, place: row * segments + segment
   int32_t* status;
 };
 
@@ -302,8 +302,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     range = RangeBegin{row * a.segments + segment, t0 - page, p, t0};
   }
   if (a.where && lane == 0 && x < a.ranges) {
-    a.where[x] = range;
-    if (x == a.ranges - 1) a.where[x + 1].begin = all;
+    put_record(a.where, x, range);
+    if (x == a.ranges - 1) a.where[4 * x + 7] = all;
   }
 
   // ---- the walk ---------------------------------------------------------------------
@@ -654,23 +654,25 @@ __global__ void __launch_bounds__(kShare == 1 ? 128 : 32 * kShare) kv8_join_kern
     if (threadIdx.x == 0) found = kMaxRanges;
     __syncthreads();
     for (int i = threadIdx.x + 1; i < a.ranges; i += 32 * kShare)
-      if (a.where[i].place == blockIdx.x && begins_inside(a.where[i])) atomicMin(&found, i);
+      if (a.where[4 * i] == blockIdx.x && begins_inside(record_of(a.where, i))) atomicMin(&found, i);
     __syncthreads();
     x = found;
     if (x == kMaxRanges) return;
   }
-  if (!cuts_first(a.where, x)) return;
-  const int64_t place = a.where[x].place, first = a.where[x].first, end = first + a.where[x].tiles;
+  const RangeBegin cut = record_of(a.where, x);
+  const int64_t before = begin_of(a.where, x - 1);
+  if (!cuts_first(cut, before)) return;
+  const int64_t place = cut.place, end = cut.first + cut.tiles;
   const int64_t row = place / a.segments, segment = place - row * a.segments;
   const int group = static_cast<int>(segment % a.groups), hg = kShare == 1 ? blockIdx.y * 4 + warp : blockIdx.y;
   if (hg >= min(kHeads, a.per_kv - group * kHeads)) return;   // kShare > 1: the whole block
   const int64_t h = segment / a.groups * a.per_kv + group * kHeads + hg;
-  const int64_t shift = a.where[x - 1].begin < first ? kHeads : 0;
+  const int64_t shift = before < cut.first ? kHeads : 0;
   auto part = [&](int i) { return static_cast<int64_t>(x - 1 + i) * 2 * kHeads + hg + (i == 0 ? shift : 0); };
   float m = -CUDART_INF_F, l = 0.0f;
   int parts = 0;
   for (int i = lane; i <= a.ranges - x; i += 32) {
-    const int64_t t0 = a.where[x - 1 + i].begin, t1 = a.where[x + i].begin;
+    const int64_t t0 = begin_of(a.where, x - 1 + i), t1 = begin_of(a.where, x + i);
     if (t0 >= end) break;
     parts = i + 1;
     if (t1 > t0) m = fmaxf(m, a.part_ml[2 * part(i)]);
@@ -684,7 +686,7 @@ __global__ void __launch_bounds__(kShare == 1 ? 128 : 32 * kShare) kv8_join_kern
   float4 o = make_float4(0, 0, 0, 0);
 #pragma unroll 8
   for (int i = kShare == 1 ? 0 : warp; i < parts; i += kShare) {
-    if (a.where[x + i].begin == a.where[x - 1 + i].begin) continue;
+    if (begin_of(a.where, x + i) == begin_of(a.where, x - 1 + i)) continue;
     const float w = exp2f(a.part_ml[2 * part(i)] - ref);
     l += a.part_ml[2 * part(i) + 1] * w;
     const float4 v = *reinterpret_cast<const float4*>(a.part + part(i) * 128 + 4 * lane);
@@ -796,7 +798,7 @@ extern "C" int64_t v1x_kv8_attend_workspace(int64_t rows, int64_t heads, int64_t
   using namespace v1x;
   if (rows <= 0 || kv_heads <= 0 || heads <= 0 || heads > 1024 || heads % kv_heads || table_pages <= 0) return 0;
   const Plan p = plan_for(rows, heads, kv_heads, table_pages);
-  return p.ranges == 1 ? 0 : (p.ranges + 1) * static_cast<int64_t>(sizeof(RangeBegin)) + p.ranges * 2 * 8 * p.tiles * (128 + 2) * 4;
+  return p.ranges == 1 ? 0 : (p.ranges + 1) * 32 + p.ranges * 2 * 8 * p.tiles * (128 + 2) * 4;
 }
 
 extern "C" int v1x_kv8_attend(const void* q, int64_t qs0, int64_t qs1, const uint8_t* k_cache, const float* k_scale,
@@ -832,8 +834,8 @@ extern "C" int v1x_kv8_attend(const void* q, int64_t qs0, int64_t qs1, const uin
                static_cast<int>(heads / kv_heads), static_cast<int>(p.groups), static_cast<int>(p.segments),
                static_cast<int>(p.ranges), scale * kLog2e, out, lse, nullptr, nullptr, nullptr, status};
   if (p.ranges > 1) {
-    a.where = static_cast<RangeBegin*>(workspace);
-    a.part = reinterpret_cast<float*>(a.where + p.ranges + 1);
+    a.where = static_cast<int64_t*>(workspace);
+    a.part = reinterpret_cast<float*>(a.where + 4 * (p.ranges + 1));
     a.part_ml = a.part + p.ranges * 2 * 8 * p.tiles * 128;
   }
   CUtensorMap k_map = {}, v_map = {};

@@ -90,7 +90,7 @@ struct LatentArgs {
   float* lse;
   float* part;       // [ranges * groups][2][16][latent][4]: four heads' values side by side; then [..][2][2][64] maxima, sums
   float* part_ml;
-  RangeBegin* where; // [ranges + 1]
+  int64_t* where;    // [ranges + 1][4]: the ranges' records
   int32_t* status;
 };
 
@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
   const int n = static_cast<int>(t1 - t0);     // tiles of the range
   Place at{static_cast<int>(sh.start.place), static_cast<int>(t0 - sh.start.first), static_cast<int>(sh.start.tiles)};
   if (tid == 0 && group == 0 && a.where) {
-    a.where[x] = sh.start;
-    if (x == a.ranges - 1) a.where[x + 1].begin = sh.all;
+    put_record(a.where, x, sh.start);
+    if (x == a.ranges - 1) a.where[4 * x + 7] = sh.all;
   }
 
   if (warp < 4) {
@@ -722,24 +722,25 @@ __global__ void __launch_bounds__(kShare == 1 ? kLatent / 2 : 32 * kShare) laten
     if (threadIdx.x == 0) found = kMaxCtas;
     __syncthreads();
     for (int i = threadIdx.x + 1; i < a.ranges; i += 32 * kShare)
-      if (a.where[i].place == blockIdx.x && begins_inside(a.where[i])) atomicMin(&found, i);
+      if (a.where[4 * i] == blockIdx.x && begins_inside(record_of(a.where, i))) atomicMin(&found, i);
     __syncthreads();
     x = found;
     if (x == kMaxCtas) return;
   }
-  if (!cuts_first(a.where, x)) return;                       // the whole block
-  const int64_t row = a.where[x].place, first = a.where[x].first, end = first + a.where[x].tiles;
-  const bool earlier = a.where[x - 1].begin < first;
+  const RangeBegin cut = record_of(a.where, x);
+  const int64_t before = begin_of(a.where, x - 1);
+  if (!cuts_first(cut, before)) return;                      // the whole block
+  const int64_t row = cut.place, end = cut.first + cut.tiles;
   // the part of range x - 1 + i, which may begin in an earlier row if i is 0
   const int64_t base = (static_cast<int64_t>(x - 1) * a.groups + h / kGroup) * 2, step = 2 * a.groups;
-  auto part = [&](int i) { return base + i * step + (i == 0 && earlier ? 1 : 0); };
-  auto live = [&](int i) { return a.where[x + i].begin > a.where[x - 1 + i].begin; };
+  auto part = [&](int i) { return base + i * step + (i == 0 && before < cut.first ? 1 : 0); };
+  auto live = [&](int i) { return begin_of(a.where, x + i) > begin_of(a.where, x - 1 + i); };
   auto four = [](const float* p) { return *reinterpret_cast<const float4*>(p); };
   const float* const ml = a.part_ml + h % kGroup;
   float4 m = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
   int parts = 0;
   for (int i = lane; i <= a.ranges - x; i += 32) {
-    if (a.where[x - 1 + i].begin >= end) break;
+    if (begin_of(a.where, x - 1 + i) >= end) break;
     parts = i + 1;
     if (!live(i)) continue;
     const float4 v = four(ml + part(i) * 2 * kGroup);
@@ -908,7 +909,7 @@ extern "C" int64_t v1x_latent_attention_workspace(int64_t rows, int64_t heads, i
   if (rows <= 0 || heads <= 0 || heads > 1024 || count <= 0 || latent <= 0) return 0;
   const Cut c = cut_for(rows, heads, count, equal != 0);
   if (c.whole || c.ranges == 1) return 0;
-  return (c.ranges + 1) * static_cast<int64_t>(sizeof(RangeBegin)) + c.ranges * ((heads + kGroup - 1) / kGroup) * 2 * kGroup * (latent + 2) * 4;
+  return (c.ranges + 1) * 32 + c.ranges * ((heads + kGroup - 1) / kGroup) * 2 * kGroup * (latent + 2) * 4;
 }
 
 extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, const void* pool, int64_t slots,
@@ -943,8 +944,8 @@ extern "C" int v1x_latent_attention(const void* q, int64_t qs0, int64_t qs1, con
                0, static_cast<int>(groups), static_cast<int>(c.ranges), static_cast<int>(c.share), c.unit, c.base, c.extra, scale * kLog2e, out,
                lse, nullptr, nullptr, nullptr, status};
   if (need) {
-    a.where = static_cast<RangeBegin*>(workspace);
-    a.part = reinterpret_cast<float*>(a.where + c.ranges + 1);
+    a.where = static_cast<int64_t*>(workspace);
+    a.part = reinterpret_cast<float*>(a.where + 4 * (c.ranges + 1));
     a.part_ml = a.part + c.ranges * groups * 2 * kGroup * latent;
   }
   V1X_CHECK_ARG(c.unit * (c.base + 1) < (int64_t(1) << 31), "latent_attention: too many tokens for one call");

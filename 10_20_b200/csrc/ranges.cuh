@@ -20,7 +20,6 @@
 namespace v1x {
 namespace attn {
 
-// [ranges + 1] of them; the last one's `begin` is the number of all tiles
 struct RangeBegin {
   int64_t place;   // the row (or the row and its segment) in which the range begins
   int64_t first;   // that row's first tile in the line
@@ -50,10 +49,23 @@ V1X_HD RangeBegin find_begin(int64_t begin, int64_t row, int64_t rows, int64_t f
 
 V1X_HD bool begins_inside(const RangeBegin& r) { return r.begin > r.first && r.begin < r.first + r.tiles; }
 
-// Range x is the first one to begin inside its row.
-V1X_HD bool cuts_first(const RangeBegin* where, int64_t x) {
-  return begins_inside(where[x]) && where[x - 1].begin <= where[x].first;
+// The range is the first one to begin inside its row; `before`: where the range before it begins.
+V1X_HD bool cuts_first(const RangeBegin& r, int64_t before) { return begins_inside(r) && before <= r.first; }
+
+// The records of all ranges, four words each, [ranges + 1] of them; of the last one only
+// `begin` is there, the number of all tiles.  (As an array of the struct the joins of
+// many rows took 72 to 84 registers instead of 60, and 100 rows of 2048 tokens 82 us
+// instead of 76.)
+V1X_HD void put_record(int64_t* where, int64_t x, const RangeBegin& r) {
+  where[4 * x] = r.place;
+  where[4 * x + 1] = r.first;
+  where[4 * x + 2] = r.tiles;
+  where[4 * x + 3] = r.begin;
 }
+V1X_HD RangeBegin record_of(const int64_t* where, int x) {
+  return RangeBegin{where[4 * x], where[4 * x + 1], where[4 * x + 2], where[4 * x + 3]};
+}
+V1X_HD int64_t begin_of(const int64_t* where, int x) { return where[4 * x + 3]; }
 
 }  // namespace attn
 }  // namespace v1x

@@ -36,7 +36,8 @@ static int batch(const std::vector<int64_t>& tiles, int64_t segments, int64_t ra
   int64_t all = 0;
   for (int64_t t : tiles) all += t * segments;
   const int64_t base = all / ranges, extra = all % ranges;
-  std::vector<RangeBegin> where(ranges + 1);
+  std::vector<int64_t> words(4 * (ranges + 1), 0);
+  int64_t* const where = words.data();
   for (int64_t x = 0; x < ranges; ++x) {
     const int64_t t0 = range_start(x, 1, base, extra);
     RangeBegin r = t0 >= all ? no_row(t0) : find_begin(t0, 0, rows, 0, [&](int64_t i) { return tiles[i] * segments; });
@@ -44,9 +45,9 @@ static int batch(const std::vector<int64_t>& tiles, int64_t segments, int64_t ra
       const int64_t p = r.tiles / segments, segment = (t0 - r.first) / p;
       r = RangeBegin{r.place * segments + segment, r.first + segment * p, p, t0};
     }
-    where[x] = r;
+    put_record(where, x, r);
   }
-  where[ranges].begin = all;
+  where[4 * ranges + 3] = all;
 
   // what has to be joined: the segments that lie in several ranges, and those ranges
   std::map<int64_t, std::vector<int64_t>> want;
@@ -55,7 +56,7 @@ static int batch(const std::vector<int64_t>& tiles, int64_t segments, int64_t ra
     for (int64_t s = 0; s < segments; ++s, line += tiles[i]) {
       std::vector<int64_t> in;
       for (int64_t x = 0; x < ranges; ++x) {
-        const int64_t t0 = where[x].begin, t1 = where[x + 1].begin;
+        const int64_t t0 = begin_of(where, x), t1 = begin_of(where, x + 1);
         if (t0 < t1 && t0 < line + tiles[i] && t1 > line) in.push_back(x);
       }
       if (in.size() > 1) want[i * segments + s] = in;
@@ -63,23 +64,23 @@ static int batch(const std::vector<int64_t>& tiles, int64_t segments, int64_t ra
 
   auto parts = [&](int64_t x) {   // of the join on behalf of range x
     std::vector<int64_t> in;
-    const int64_t end = where[x].first + where[x].tiles;
-    for (int64_t i = 0; i <= ranges - x && where[x - 1 + i].begin < end; ++i)
-      if (where[x + i].begin > where[x - 1 + i].begin) in.push_back(x - 1 + i);
+    const int64_t end = record_of(where, x).first + record_of(where, x).tiles;
+    for (int64_t i = 0; i <= ranges - x && begin_of(where, x - 1 + i) < end; ++i)
+      if (begin_of(where, x + i) > begin_of(where, x - 1 + i)) in.push_back(x - 1 + i);
     return in;
   };
   int bad = 0;
   std::map<int64_t, std::vector<int64_t>> one, sixteen;
   for (int64_t x = 1; x < ranges; ++x)
-    if (cuts_first(where.data(), x)) {
-      if (one.count(where[x].place)) ++bad;
-      one[where[x].place] = parts(x);
+    if (cuts_first(record_of(where, x), begin_of(where, x - 1))) {
+      if (one.count(where[4 * x])) ++bad;
+      one[where[4 * x]] = parts(x);
     }
   for (int64_t place = 0; place < rows * segments; ++place) {
     int64_t found = ranges;
     for (int64_t i = ranges - 1; i >= 1; --i)
-      if (where[i].place == place && begins_inside(where[i])) found = i;
-    if (found < ranges && cuts_first(where.data(), found)) sixteen[place] = parts(found);
+      if (where[4 * i] == place && begins_inside(record_of(where, i))) found = i;
+    if (found < ranges && cuts_first(record_of(where, found), begin_of(where, found - 1))) sixteen[place] = parts(found);
   }
   if (bad || one != want || sixteen != want) {
     std::printf("%s: %lld rows, %lld segments, %lld tiles, %lld ranges: %zu to join, %zu and %zu joined\n", what,
