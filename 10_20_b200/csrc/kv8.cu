@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(128) kv8_store_kernel(const __grid_constant__ 
 //     lane g takes 16 g .. 16 g + 15; with the buffers' 128-byte swizzle every 16-byte
 //     read is free of conflicts;
 // 64 rows of 1-16 K tokens, 32 heads over 4: 103 us, 5.5 TB/s (the join about 8 of them);
-// one row of 4097 tokens 13 us.
+// 64 heads over 4 157 us, where the two-tile kernel fills 255 registers and spills; one
+// row of 4097 tokens 13 us.
 //   * the query is held in f16 under a power of two per head that puts its largest
 //     value in [1, 2); the weights, up to 2^15, are rounded to f16 once, sums stay in 32 bits; a
 //     page's output is added under its value scale in 32 bits, so scales of any size
@@ -716,7 +717,7 @@ Plan plan_for(int64_t rows, int64_t heads, int64_t kv_heads, int64_t table_pages
   Plan p;
   const int64_t per = heads / kv_heads;
   // one 8-column operand where it holds all the heads, else two (64 rows of 1-16 K
-  // tokens: 8 heads a K/V head 103 us with one, 169 with two; 16 heads 184 and 159)
+  // tokens: 8 heads a K/V head 103 us with one, 169 with two; 16 heads 184 and 157)
   p.tiles = per <= 8 ? 1 : 2;
   p.groups = (per + 8 * p.tiles - 1) / (8 * p.tiles);
   p.segments = kv_heads * p.groups;

@@ -711,7 +711,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_kernel(const __grid_consta
 //     rows (grid x) spread over all ranges.
 // Both kernels: one row of 131072 tokens 111 us with one, 53.5 with sixteen (62 with
 // four and a head a warp); 512 tokens 15.4 and 13.1; 12 rows of 2048 30 and 38; 48
-// ragged rows 107 and 123.
+// ragged rows 107 and 123.  Around the rule's bound of 512 rows x heads, one and
+// sixteen: 192 (12 rows, 16 heads) 28.7 and 28.2; 256 (4 rows of 4096, 64 heads) 38.0
+// and 27.2, (of 16384) 47.9 and 40.6; 432 (18 rows of 2048, 24 heads) 25.7 and 29.7; 448
+// (7 rows of 8192) 40.6 and 42.3; 512 (8 rows of 2048) 31.3 and 31.2, (of 8192) 42.9 and
+// 44.9; 576 (9 rows of 2048) 28.7 and 32.0; 768 (12 rows of 8192) 50.5 and 57.8.
 template <typename T, int kLatent, int kShare>
 __global__ void __launch_bounds__(kShare == 1 ? kLatent / 2 : 32 * kShare) latent_join_kernel(const __grid_constant__ LatentArgs a) {
   wait_for_previous();

@@ -85,7 +85,8 @@ def attend(q, k_cache, k_scale, v_cache, v_scale, table, lens, scale, out=None, 
     """Attention of q [rows, heads, 128] (bfloat16 / float16) over the cache:
     s[h, j] = scale * q[r, h, :] . k_j of head h // (heads / kv_heads), token j < lens[r]
     in page ``table[r, j // 64]``.  lens int32 [rows] (at most pages * 64 count;
-    negative is 0).  The tokens of a page outside the cache are no tokens."""
+    negative is 0).  The tokens of a page outside the cache are no tokens.  Below
+    2^25 pages x kv_heads and table columns, at most 2^34 rows x kv_heads x columns."""
     pages, kv_heads = _cache(k_cache, k_scale, v_cache, v_scale)
     code = _DTYPES.get(q.dtype)
     require(code is not None and q.dim() == 3 and q.shape[2] == 128, "q: [rows, heads, 128] bfloat16 or float16")

@@ -164,7 +164,8 @@ def attend_prompt(q, k, k_rope, v, offsets, scale, kv_offsets=None, out=None, ls
     shared by the heads, dr = 64, or None for dr = 0; all of one type
     (bfloat16 / float16), unit inner stride, rows 16-byte aligned -- views of
     one projection's output or of pool rows are taken as they are.  offsets and
-    kv_offsets: int32 [requests + 1], non-decreasing, within the tokens.  Rows
+    kv_offsets: int32 [requests + 1], non-decreasing, within the tokens; tokens /
+    256 + requests is at most 65535.  Rows
     of q that no request covers are not written in out and lse.  A NaN or an
     infinity among a request's values also reaches queries that come before it
     (0 times it is NaN); other requests' keys and values are never read."""
