@@ -39,6 +39,7 @@
 #include <type_traits>
 
 #include "attention.cuh"
+#include "ring.cuh"
 #include "sm100.cuh"
 
 namespace v1x {
@@ -380,7 +381,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(pending);
     };
-    int slot = 0, turn = 0, boxes[kSlots] = {-1, -1, -1};   // boxes: the turn of a slot's last TMA load
+    int slot = 0, turn = 0;
+    LastBoxes<kSlots> boxes;
     for (int u = 0; u < 2 * n; ++u) {
       const int j = u >> 1, rope = j % kRopeSlots;
       const bool keys = (u & 1) == 0;
@@ -411,9 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kSlots; ++i)
-          if (i == slot) boxes[i] = turn;
+        boxes.box(slot, turn);
         if (++slot == kSlots) {
           slot = 0;
           ++turn;
@@ -429,6 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         report();
       }
       pending = &sh.full[slot];
+      boxes.copy(slot);
       if (++slot == kSlots) {
         slot = 0;
         ++turn;
@@ -436,9 +437,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     cp_async_wait_all();
     if (pending) report();
-    if (*reinterpret_cast<volatile int*>(&sh.abort) && half == 0)   // boxes that are under way land before the CTA ends
+    // boxes that are under way land before the CTA ends, whoever gives up, now or later
+    if (half == 0)
+#pragma unroll
       for (int i = 0; i < kSlots; ++i)
-        if (boxes[i] >= 0) mbar_wait(&sh.full[i], boxes[i] & 1, &sh.zero, kWaitNs);
+        if (boxes.turns[i] >= 0) mbar_wait(&sh.full[i], boxes.turns[i] & 1, &sh.zero, kWaitNs);
   }
   __syncthreads();
   if (warp == 8) {

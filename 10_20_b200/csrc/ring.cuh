@@ -35,5 +35,27 @@ struct RingState {
   }
 };
 
+// The box that each of a ring's buffers got last, where boxes and plain copies take turns
+// in it: what may still be under way once all have been sent.
+template <int kSlots>
+struct LastBoxes {
+  int turns[kSlots];     // the buffer's turn, whose phase the box ends; -1: no box since the last copy
+
+  V1X_HD LastBoxes() {
+    for (int& t : turns) t = -1;
+  }
+  V1X_HD void box(int slot, int turn) { set(slot, turn); }
+  // A copy: its buffer was free, so the box before it has landed.
+  V1X_HD void copy(int slot) { set(slot, -1); }
+
+  V1X_HD void set(int slot, int turn) {
+#ifdef __CUDA_ARCH__
+#pragma unroll
+#endif
+    for (int i = 0; i < kSlots; ++i)
+      if (i == slot) turns[i] = turn;
+  }
+};
+
 }  // namespace attn
 }  // namespace v1x

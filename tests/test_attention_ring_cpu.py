@@ -1,11 +1,11 @@
-"""CPU: the 8-bit attention's ring of buffers when a wait gives up (csrc/ring.cuh).
+"""CPU: the attention kernels' rings of buffers when a wait gives up (csrc/ring.cuh).
 
-A program built from the header walks pages as a warp does -- keys, values and the next
-page's keys in three buffers, some pages outside the cache -- over barriers that count
-boxes, with every wait in turn giving up while its box is still under way, and later
-ones giving up too or not.  The warp ends its page, or leaves it at once.  No box may
-be sent to a buffer that waits for one, every wait has to be for the phase of the box
-under way, and all boxes have to have landed at the end."""
+A program built from the header walks pages as a warp of the 8-bit attention does --
+keys, values and the next page's keys in three buffers, some pages outside the cache --
+over barriers that count boxes, with every wait in turn giving up while its box is still
+under way, and later ones giving up too or not.  The warp ends its page, or leaves it at
+once.  No box may be sent to a buffer that waits for one, every wait has to be for the
+phase of the box under way, and all boxes have to have landed at the end."""
 import shutil
 import subprocess
 from pathlib import Path
@@ -102,15 +102,59 @@ int main() {
 """
 
 
-def test_a_wait_that_gives_up_leaves_no_box_behind(tmp_path):
+# The prompt attention's producer: whole tiles by boxes, a last partial one by copies, into
+# buffers in turn; the consumers free them in order, up to a place where they give up.
+PROMPT = r"""
+#include <cstdio>
+
+#include "ring.cuh"
+
+int main() {
+  constexpr int kSlots = 3;
+  int bad = 0;
+  for (int whole = 0; whole <= 14; ++whole)
+    for (int rest = 0; rest <= 2; rest += 2)            // keys and values of the partial tile
+      for (int freed = 0; freed <= whole + rest; ++freed)       // loads whose buffers become free
+        for (int landed = freed; landed <= whole + rest; ++landed) {   // loads that have landed at the end
+          v1x::attn::LastBoxes<kSlots> last;
+          int phases[kSlots] = {0, 0, 0}, sent = 0;     // phases: loads of a buffer that have landed
+          int box_in[kSlots] = {-1, -1, -1};            // the load whose box a buffer got last
+          for (int u = 0; u < whole + rest; ++u) {
+            const int slot = u % kSlots, turn = u / kSlots;
+            if (u >= kSlots && u - kSlots >= freed) break;      // the wait for the buffer gives up
+            if (u < whole) {
+              last.box(slot, turn);
+              box_in[slot] = u;
+            } else {
+              last.copy(slot);
+              box_in[slot] = -1;
+            }
+            ++sent;
+          }
+          for (int u = 0; u < sent && u < landed; ++u) ++phases[u % kSlots];
+          for (int i = 0; i < kSlots; ++i) {
+            const int turn = last.turns[i];
+            // a box under way is waited for, in its own phase; a wait's phase is the current or the last one
+            if (box_in[i] >= landed && turn != box_in[i] / kSlots) ++bad;
+            if (turn >= 0 && phases[i] != turn && phases[i] != turn + 1) ++bad;
+          }
+        }
+  std::printf("%d faults\n", bad);
+  return bad != 0;
+}
+"""
+
+
+@pytest.mark.parametrize("program", [PROGRAM, PROMPT], ids=["decode", "prompt"])
+def test_a_wait_that_gives_up_leaves_no_box_behind(tmp_path, program):
     cxx = shutil.which("g++") or shutil.which("c++")
     if cxx is None:
         pytest.skip("no host compiler")
     source = tmp_path / "ring.cpp"
-    source.write_text(PROGRAM)
-    program = tmp_path / "ring"
-    built = subprocess.run([cxx, "-std=c++17", "-O1", "-x", "c++", "-I", str(CSRC), str(source), "-o", str(program)],
+    source.write_text(program)
+    binary = tmp_path / "ring"
+    built = subprocess.run([cxx, "-std=c++17", "-O1", "-x", "c++", "-I", str(CSRC), str(source), "-o", str(binary)],
                            capture_output=True, text=True)
     assert built.returncode == 0, built.stderr
-    ran = subprocess.run([str(program)], capture_output=True, text=True, timeout=120)
+    ran = subprocess.run([str(binary)], capture_output=True, text=True, timeout=120)
     assert ran.returncode == 0, ran.stdout
